@@ -19,6 +19,8 @@ ABI_VERSION = 3  # iris_abi_version() of the library these signatures describe
 F32, BF16 = 0, 1
 EPI_NONE, EPI_SILU_MUL, EPI_SILU = 0, 1, 2
 ACT_NONE, ACT_SILU = 0, 1
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+ROTARY_TURN, ROTARY_TO_ROWS = 1, 2
 E_INVALID, E_LAUNCH, E_UNSUPPORTED = -1, -2, -3
 
 P = c_void_p
@@ -42,6 +44,11 @@ _SIGNATURES: dict[str, list] = {
     "iris_gemm_force_tile": [c_int],
     "iris_flash_attn_force_variant": [c_int],
     "iris_flash_attn_masked": [P, P, P, c_int, c_int, c_int, c_long, c_long, c_float, P, P, c_long, c_long, P],
+    "iris_rotary": [c_int, P, P, P, P, P, P, P, c_int, c_int, c_long, c_int, P, c_int, c_long, P, c_int, c_long, P, c_int,
+                    c_int, c_float, c_int, P],
+    "iris_window_attn": [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_long, c_long, c_long, c_long, c_int, P, c_int, P,
+                         c_int, c_long, P, c_long, c_float, P],
+    "iris_gemv_w4": [c_int, P, P, c_int, P, c_int, P, c_int, c_int, P, c_int, P, P, P, P, c_int, c_int, c_int, P],
     "iris_text_key_mask": [P, c_int, c_long, c_int, c_long, c_long, P, P],
     "iris_layer_attention": [P, P, c_long, c_int, c_int, c_int, c_float, P],
     "iris_layer_pool": [P, P, P, P, c_long, c_int, c_int, P, c_int, P],

@@ -62,6 +62,21 @@ class _Check:
         return self
 
 
+_INT_KINDS = {torch.int32: 1, torch.int64: 3}
+
+
+def _on_current_device(op: str, first: torch.Tensor, *rest: torch.Tensor | None) -> None:
+    """All tensors on the GPU that the call's stream belongs to (the current one)."""
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError(f"{op}: the HIP kernels need GPU tensors (there is no CPU path)")
+    for t in rest:
+        if t is not None and t.device != device:
+            raise ValueError(f"{op}: tensors on {device} and on {t.device}: all must be on one GPU")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"{op}: tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
 def _mod_rows(vector: torch.Tensor, batch: int, width: int) -> tuple[torch.Tensor, int]:
     """A ``[B, 1, D]`` slice of a modulation vector as FP32 rows the kernels read with 16-byte
     loads: returned in place when its rows are unit-stride and 16-byte aligned (slices of the
@@ -126,6 +141,128 @@ def qk_norm_rope(
         float(eps), L.stream(),
     )
     return out
+
+
+def _rotary(op, turned, plain, outs, positions, freqs, rows, layout, factor, transpose) -> None:
+    """``iris_rotary`` of the ``turned`` tensors and the ``plain`` one (or None) into ``outs``, in that order;
+    with ``rows``, all outputs but the first go to them."""
+    xs = [*turned, plain] if plain is not None else turned
+    first = xs[0]
+    if layout not in L.ROTARY_LAYOUTS:
+        raise ValueError(f"{op}: layout must be 'half' or 'interleaved', got {layout!r}")
+    if first.dim() != 4:
+        raise ValueError(f"{op}: heads must be [B, N, H, D]")
+    batch, tokens, _, dim = first.shape
+    pairs = freqs.numel()
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 0 < 2 * pairs <= dim or dim % 2:
+        raise ValueError(f"{op}: freqs must be contiguous FP64, one per rotated pair of the (even) head width {dim}")
+    x_strides, out_strides, heads, flags, out_rows = [], [], [], [], []
+    for i, (x, out) in enumerate(zip(xs, outs)):
+        if (x.dim() != 4 or x.shape[:2] != (batch, tokens) or x.shape[3] != dim or x.dtype != first.dtype
+                or (x.stride(3) != 1 and dim > 1)):
+            raise ValueError(f"{op}: heads must be [{batch}, {tokens}, H, {dim}] of one dtype with unit stride in a head")
+        to_rows = rows is not None and i > 0
+        h = x.shape[2]
+        if (out.dim() != 4 or out.shape[:2] != (batch, h) or out.shape[3] != dim or out.dtype != x.dtype
+                or out.stride(3) != 1 or (not to_rows and out.shape[2] != tokens)):
+            raise ValueError(f"{op}: output {i} must be {x.dtype} [{batch}, {h}, "
+                             f"{'rows' if to_rows else tokens}, {dim}] with unit stride in a head")
+        xs_, os_ = x.stride(), out.stride()
+        if _span_overlaps(x, out) and (to_rows or x.data_ptr() != out.data_ptr()
+                                       or (xs_[0], xs_[2], xs_[1]) != os_[:3]):
+            raise ValueError(f"{op}: output {i} must be its input itself (as [B, H, N, D]) or lie apart from it")
+        if out.shape[2] > 1 and os_[2] == 0 or h > 1 and os_[1] == 0 or batch > 1 and os_[0] == 0:
+            raise ValueError(f"{op}: output {i} is an expanded tensor")
+        x_strides += xs_[:3]
+        out_strides += os_[:3]
+        heads.append(h)
+        flags.append((L.ROTARY_TURN if i < len(turned) else 0) | (L.ROTARY_TO_ROWS if to_rows else 0))
+        out_rows.append(out.shape[2])
+    strides = []
+    for name, index in (("positions", positions), ("rows", rows)):
+        if index is None:
+            strides.append((0, 0))
+            continue
+        kind = _INT_KINDS.get(index.dtype, 0)
+        if (kind == 0 or index.shape not in ((tokens,), (batch, tokens)) or (tokens > 1 and index.stride(-1) != 1)):
+            raise ValueError(f"{op}: {name} must be int32 or int64 [{batch}, {tokens}] or [{tokens}] with unit stride")
+        strides.append((kind, index.stride(0) if index.dim() == 2 else 0))
+    dtype = L.dtype_code(first.dtype)
+    _on_current_device(op, *xs, *outs, positions, freqs, rows)
+    P = L.pointer_array
+    L.call("iris_rotary", len(xs), P([x.data_ptr() for x in xs]), L.long_array(x_strides),
+           P([o.data_ptr() for o in outs]), L.long_array(out_strides), L.int_array(heads), L.int_array(flags),
+           L.long_array(out_rows), dtype, batch, tokens, dim, positions.data_ptr(), *strides[0],
+           L.ptr(rows), *strides[1], freqs.data_ptr(), pairs, L.ROTARY_LAYOUTS[layout], float(factor), bool(transpose),
+           L.stream())
+
+
+def _span_overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    if not a.numel() or not b.numel():
+        return False
+    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
+    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
+def rotary(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions: torch.Tensor,
+    freqs: torch.Tensor,
+    layout: str = "half",
+    factor: float = 1.0,
+    transpose: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotary positions of query and key heads and their ``[B, N, H, D] -> [B, H, N, D]`` layout, in one launch.
+
+    ``q`` / ``k`` (or None): FP32 or BF16 ``[B, N, H, D]`` and ``[B, N, H_kv, D]`` views with unit stride
+    inside a head (a packed projection's heads); ``positions``: int32 or int64 ``[B, N]`` or ``[N]``, any
+    value; ``freqs``: FP64 ``[pairs]`` angles per position (``tables.rotary_frequencies``). The first
+    ``2 * pairs`` elements of a head turn, in pairs ``(i, i + pairs)`` (``layout="half"``) or
+    ``(2 i, 2 i + 1)`` (``"interleaved"``), scaled by ``factor``; the rest are copied. Angles are formed
+    in FP64, the rotation in FP32. ``transpose=True`` turns the other way: the gradient with regard to the
+    inputs of the call without it. ``q_out`` / ``k_out``: ``[B, H, N, D]`` views of any strides with unit
+    stride inside a head; the input itself, transposed to that shape, is rotated in place."""
+    turned = [q] if k is None else [q, k]
+    for x in turned:
+        if x.dim() != 4:
+            raise ValueError("rotary: heads must be [B, N, H, D]")
+    outs = [o if o is not None else x.new_empty(x.shape[0], x.shape[2], x.shape[1], x.shape[3])
+            for x, o in zip(turned, (q_out, k_out))]
+    _rotary("rotary", turned, None, outs, positions, freqs, None, layout, factor, transpose)
+    return outs[0], (outs[1] if k is not None else None)
+
+
+def rotary_store(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    freqs: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    rows: torch.Tensor | None = None,
+    layout: str = "half",
+    factor: float = 1.0,
+    q_out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``rotary`` of ``q`` and ``k`` with ``k`` and ``v`` leaving for caches, in one launch; returns the
+    rotated queries ``[B, H, N, D]``.
+
+    ``k_cache`` / ``v_cache``: ``[B, H_kv, N_max, D]`` views of any strides with unit stride inside a head
+    (as ``window_attention`` reads them). Token ``t`` of item ``b`` goes to cache row ``rows[b, t]`` (int32
+    or int64, ``[B, N]`` or ``[N]``; default ``positions``), and nowhere if that row does not exist: -1 marks
+    padding. All other rows stay as they are. The rows of one item must differ from each other."""
+    if q.dim() != 4:
+        raise ValueError("rotary_store: heads must be [B, N, H, D]")
+    if q_out is None:
+        q_out = q.new_empty(q.shape[0], q.shape[2], q.shape[1], q.shape[3])
+    _rotary("rotary_store", [q, k], v, [q_out, k_cache, v_cache], positions, freqs,
+            positions if rows is None else rows, layout, factor, False)
+    return q_out
 
 
 def rms_norm_modulate(
@@ -634,6 +771,88 @@ def flash_attention_masked(q, k, vt, n: int, key_mask: torch.Tensor, out: torch.
 _MASK_KINDS = {torch.bool: 0, torch.uint8: 0, torch.int8: 0, torch.int32: 1, torch.float32: 2, torch.int64: 3}
 
 
+def window_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    window: int | None = None,
+    sinks: int = 0,
+    causal: bool = True,
+    lengths: torch.Tensor | None = None,
+    starts: torch.Tensor | int | None = None,
+    key_mask: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``softmax(q k^T * scale) v`` with a sliding window and a few first keys that stay visible, for whole
+    prompts and for one or a few queries over a cache: BF16 ``[B, Nq, H * 128]``.
+
+    ``q``: BF16 ``[B, H, Nq, 128]``, ``k`` / ``v``: BF16 ``[B, H_kv, Nk, 128]`` (``H`` a multiple of
+    ``H_kv``), views of any strides that are multiples of 8 elements (a packed projection's heads, a
+    cache), 16-byte aligned, unit stride inside a head. Query ``t`` of item ``b`` is at position
+    ``starts[b] + t`` (default: the last ``Nq`` of the item's keys, ``lengths[b] - Nq``) and sees key
+    ``j < lengths[b]`` (default ``Nk``) where
+
+    - ``j <= position``, if ``causal``, and
+    - ``|position - j| < window``, or ``j < sinks``, or ``window`` is None, and
+    - ``key_mask[b, j]`` (bool or uint8 ``[B, Nk]``), if given.
+
+    A query that sees nothing gives 0. Keys that no query sees may hold anything; a query's result does
+    not depend on keys it does not see, infinities and NaN among them. ``scale`` defaults to
+    ``128 ** -0.5``; ``out``: BF16 ``[B, Nq, H * 128]``, unit column stride."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("window_attention: q must be [B, H, Nq, 128], k and v [B, H_kv, Nk, 128] of one shape")
+    batch, heads, n_q, hd = q.shape
+    kv_heads, n_k = k.shape[1], k.shape[2]
+    if hd != HEAD_DIM or k.shape[0] != batch or k.shape[3] != HEAD_DIM or kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"window_attention: q {tuple(q.shape)} and k / v {tuple(k.shape)} do not match: one batch, "
+                         "128-wide heads, a multiple of K/V heads")
+    bf16 = torch.bfloat16
+    if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
+        raise ValueError("window_attention: works on BF16")
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if qs[3] != 1 or ks[3] != 1 or vs[3] != 1:
+        raise ValueError("window_attention: heads must have unit stride")
+    if (window is not None and window < 1) or sinks < 0:
+        raise ValueError(f"window_attention: window must be at least 1 (or None) and sinks nonnegative, got {window}, {sinks}")
+    lengths_kind = starts_kind = start = mask_stride = 0
+    if lengths is not None:
+        lengths_kind = _INT_KINDS.get(lengths.dtype, 0)
+        if lengths_kind == 0 or lengths.shape != (batch,) or not lengths.is_contiguous():
+            raise ValueError(f"window_attention: lengths must be contiguous int32 or int64 [{batch}]")
+    if isinstance(starts, torch.Tensor):
+        starts_kind = _INT_KINDS.get(starts.dtype, 0)
+        if starts_kind == 0 or starts.shape != (batch,) or not starts.is_contiguous():
+            raise ValueError(f"window_attention: starts must be an int or contiguous int32 or int64 [{batch}]")
+    elif starts is not None:
+        starts_kind, start, starts = 4, int(starts), None
+        if abs(start) >= 1 << 60:
+            raise ValueError("window_attention: starts must lie within 2^60")
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (batch, n_k) or (
+                n_k > 1 and key_mask.stride(1) != 1):
+            raise ValueError(f"window_attention: key_mask must be bool or uint8 [{batch}, {n_k}] with unit column stride")
+        mask_stride = key_mask.stride(0)
+    width = heads * HEAD_DIM
+    if out is not None:
+        if out.dtype != bf16 or out.shape != (batch, n_q, width) or out.stride(2) != 1:
+            raise ValueError(f"window_attention: out must be BF16 [{batch}, {n_q}, {width}] with unit column stride")
+        out_strides = out.stride()[:2]
+        if (n_q > 1 and out_strides[1] < width) or (batch > 1 and out_strides[0] < width):
+            raise ValueError("window_attention: out's rows overlap")
+        if any(_span_overlaps(out, t) for t in (q, k, v)):
+            raise ValueError("window_attention: out must lie apart from q, k and v")
+    _on_current_device("window_attention", q, k, v, lengths, starts, key_mask, out)
+    if out is None:
+        out = torch.empty(batch, n_q, width, device=q.device, dtype=bf16)
+        out_strides = (n_q * width, width)
+    L.call("iris_window_attn", q.data_ptr(), L.long_array(qs[:3]), k.data_ptr(), L.long_array(ks[:3]), v.data_ptr(),
+           L.long_array(vs[:3]), out.data_ptr(), L.long_array(out_strides), batch, heads, kv_heads, n_q, n_k,
+           min(window or 0, 1 << 60), min(sinks, 1 << 60), bool(causal), L.ptr(lengths), lengths_kind, L.ptr(starts), starts_kind, start,
+           L.ptr(key_mask), mask_stride, HEAD_DIM ** -0.5 if scale is None else float(scale), L.stream())
+    return out
+
+
 def text_key_mask(mask: torch.Tensor, n: int, out: torch.Tensor) -> torch.Tensor:
     """``mask[:, :n].bool()`` as the zero-padded uint8 ``[B, N_pad]`` key mask of ``flash_attention_masked``."""
     check = _Check("text_key_mask", mask, out)
@@ -756,6 +975,110 @@ def gemv_pair(weights, x: torch.Tensor, biases, outs, extra_biases, in_silu: boo
         L.int_array([e.shape[0] for e in extra_biases]), P([L.ptr(o) for o in outs]),
         L.ACT_SILU if in_silu else L.ACT_NONE, L.ACT_NONE, L.stream(),
     )
+
+
+def pack_w4(weight: torch.Tensor, group: int = 64, symmetric: bool = True,
+            scales_dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``(codes, scales, zeros)`` of ``gemv_w4``: ``weight`` ``[N, K]`` rounded to 4 bits in groups of ``group``
+    along K. ``symmetric``: codes around 8, scale the group's largest magnitude / 7, ``zeros`` None; else codes
+    0..15 over the group's range (0 included), with the zero point rounded. Codes are chosen for the scales as
+    stored."""
+    _Check("pack_w4")(weight.dim() == 2 and weight.shape[1] % 32 == 0 and group > 0 and group % 32 == 0,
+                      "takes [N, K] weights with K and group multiples of 32")
+    n, k = weight.shape
+    groups = -(-k // group)
+    w = torch.nn.functional.pad(weight.float(), (0, groups * group - k)).view(n, groups, group)
+    if symmetric:
+        scales = (w.abs().amax(-1) / 7).to(scales_dtype)
+        zero = torch.full_like(scales, 8, dtype=torch.float32)
+    else:
+        low, high = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+        scales = ((high - low) / 15).to(scales_dtype)
+        step = torch.where(scales > 0, scales.float(), 1.0)
+        zero = (-low / step).round().clamp(0, 15)
+    step = torch.where(scales > 0, scales.float(), 1.0)
+    codes = (w / step[..., None] + zero[..., None]).round().clamp(0, 15).to(torch.uint8).view(n, -1)[:, :k]
+    return (codes[:, 0::2] | codes[:, 1::2] << 4).contiguous(), scales, None if symmetric else zero.to(torch.uint8)
+
+
+def _w4_checks(op: str, codes, scales, zeros, x, bias, extra_bias, out, group: int) -> int:
+    """Checks one product of ``gemv_w4``; returns the number of its extra biases."""
+    if x.dim() != 2 or codes.dim() != 2:
+        raise ValueError(f"{op}: takes [B, K] inputs and [N, K / 2] codes")
+    batch, k = x.shape
+    n = codes.shape[0]
+    if codes.dtype != torch.uint8 or codes.shape[1] * 2 != k or not codes.is_contiguous():
+        raise ValueError(f"{op}: codes must be contiguous uint8 [N, {k} / 2], two weights a byte")
+    if group <= 0 or group % 32:
+        raise ValueError(f"{op}: group must be a multiple of 32 (got {group})")
+    groups = (n, -(-k // group))
+    if scales.shape != groups or not scales.is_contiguous():
+        raise ValueError(f"{op}: scales must be contiguous {groups}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != groups or not zeros.is_contiguous()):
+        raise ValueError(f"{op}: zeros must be contiguous uint8 {groups}")
+    if not x.is_contiguous():
+        raise ValueError(f"{op}: x must be contiguous")
+    for name, t, shape in (("bias", bias, (n,)), ("extra_bias", extra_bias, None)):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()
+                              or (t.shape != shape if shape else t.dim() != 2 or t.shape[1] != n or t.shape[0] == 0)):
+            raise ValueError(f"{op}: {name} must be contiguous FP32 {'[N]' if shape else '[J, N]'}")
+    n_extra = 0 if extra_bias is None else extra_bias.shape[0]
+    if out.shape != ((n_extra, batch, n) if n_extra else (batch, n)) or not out.is_contiguous():
+        raise ValueError(f"{op}: out must be contiguous {(n_extra, batch, n) if n_extra else (batch, n)}")
+    if _span_overlaps(out, x):
+        raise ValueError(f"{op}: out must lie apart from x")
+    _on_current_device(op, codes, scales, zeros, x, bias, extra_bias, out)
+    return n_extra
+
+
+def gemv_w4(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    x: torch.Tensor,
+    bias: torch.Tensor | None,
+    out: torch.Tensor,
+    group: int = 64,
+    zeros: torch.Tensor | None = None,
+    extra_bias: torch.Tensor | None = None,
+    in_silu: bool = False,
+    out_silu: bool = False,
+) -> torch.Tensor:
+    """``gemv`` with 4-bit weights and group scales: ``out = act(act_in(x) W^T + bias)`` for rows ``x`` (FP32 or
+    BF16 ``[B, K]``) and ``W[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k // group])``.
+
+    ``codes``: uint8 ``[N, K / 2]``, the even k of a pair in the low half of its byte (``pack_w4``);
+    ``scales``: FP32 or BF16 ``[N, ceil(K / group)]``; ``zeros``: uint8 of that shape with values 0..15, or
+    None for 8 everywhere. K and ``group`` are multiples of 32; the last group may be short. Sums are FP32 and,
+    for FP32 inputs, of FP32 products. ``bias`` FP32 ``[N]``; ``out`` FP32 or BF16 ``[B, N]``; with
+    ``extra_bias`` (``[J, N]``) ``out[j] = y + extra_bias[j]`` (``out``: ``[J, B, N]``)."""
+    n_extra = _w4_checks("gemv_w4", codes, scales, zeros, x, bias, extra_bias, out, group)
+    batch, k = x.shape
+    P = L.pointer_array
+    L.call("iris_gemv_w4", 1, P([codes.data_ptr()]), P([scales.data_ptr()]), L.dtype_code(scales.dtype),
+           P([L.ptr(zeros)]), group, x.data_ptr(), L.dtype_code(x.dtype), batch, L.int_array([codes.shape[0]]), k,
+           P([L.ptr(bias)]), P([L.ptr(extra_bias)]), L.int_array([n_extra]), P([out.data_ptr()]),
+           L.dtype_code(out.dtype), L.ACT_SILU if in_silu else L.ACT_NONE, L.ACT_SILU if out_silu else L.ACT_NONE,
+           L.stream())
+    return out
+
+
+def gemv_w4_pair(codes, scales, x: torch.Tensor, biases, outs, group: int = 64, zeros=(None, None),
+                 extra_biases=(None, None), in_silu: bool = False, out_silu: bool = False) -> None:
+    """Two ``gemv_w4`` of the same inputs in one launch (the image and text adaLN cores); same results as the
+    two calls. Scales, and outputs, share a dtype."""
+    lists = (codes, scales, biases, outs, zeros, extra_biases)
+    _Check("gemv_w4_pair")(all(len(items) == 2 for items in lists), "takes two products")
+    n_extra = [_w4_checks("gemv_w4_pair", c, s, z, x, b, e, o, group)
+               for c, s, b, o, z, e in zip(*lists)]
+    _Check("gemv_w4_pair")(scales[0].dtype == scales[1].dtype and outs[0].dtype == outs[1].dtype,
+                           "scales or outputs differ in dtype")
+    P = L.pointer_array
+    L.call("iris_gemv_w4", 2, P([c.data_ptr() for c in codes]), P([s.data_ptr() for s in scales]),
+           L.dtype_code(scales[0].dtype), P([L.ptr(z) for z in zeros]), group, x.data_ptr(), L.dtype_code(x.dtype),
+           x.shape[0], L.int_array([c.shape[0] for c in codes]), x.shape[1], P([L.ptr(b) for b in biases]),
+           P([L.ptr(e) for e in extra_biases]), L.int_array(n_extra), P([o.data_ptr() for o in outs]),
+           L.dtype_code(outs[0].dtype), L.ACT_SILU if in_silu else L.ACT_NONE, L.ACT_SILU if out_silu else L.ACT_NONE,
+           L.stream())
 
 
 def timestep_gemv(t: torch.Tensor, freqs: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, out: torch.Tensor,

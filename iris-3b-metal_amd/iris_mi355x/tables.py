@@ -6,6 +6,7 @@ and kept on the device, as the reference engine does (src/iris_metal/model.py:14
 - the pixel stage's fixed 2-D sincos position table, stored separably as ``[W, 8]`` (x half)
   and ``[H, 8]`` (y half) since each half depends on one coordinate
   (src/iris3b/nn/embeddings.py:269-288);
+- the frequencies of ``kernels.rotary``, plain or scaled for long contexts;
 - the timestep frequency bank ``exp(-ln(P) k / n)`` (src/iris3b/nn/embeddings.py:41-45).
 """
 
@@ -49,6 +50,36 @@ def rope_1d_angles(head_dim: int, length: int, theta: float) -> torch.Tensor:
     freqs = 1.0 / theta ** (torch.arange(0, head_dim, 2)[: head_dim // 2].float() / head_dim)
     ang = torch.outer(torch.arange(length).float(), freqs)
     return torch.polar(torch.ones_like(ang), ang)
+
+
+def rotary_frequencies(dim: int, theta: float, device, scaling: str = "none", scale: float = 1.0,
+                       trained: int = 4096, slow: float = 1.0, fast: float = 32.0) -> tuple[torch.Tensor, float]:
+    """``(freqs, factor)`` of ``kernels.rotary``: FP64 ``[dim / 2]`` angles per position of the pairs of a
+    ``dim``-wide rotated part, ``theta ** (-2 i / dim)``, and the factor on the rotated values.
+
+    For contexts ``scale`` times the ``trained`` positions: ``"linear"`` divides every angle by ``scale``;
+    ``"ntk"`` raises the base so that the slowest pair is divided by ``scale`` and the fastest stays;
+    ``"by_parts"`` keeps pairs that turn at least ``fast`` times over the trained positions, divides those
+    that turn at most ``slow`` times by ``scale``, blends linearly in the number of turns between them, and
+    sets the factor to ``0.1 ln(scale) + 1`` (it meets itself in q k: the scores' temperature)."""
+    if dim <= 0 or dim % 2:
+        raise ValueError(f"rotary_frequencies: the rotated width must be even and positive, got {dim}")
+    if scaling not in ("none", "linear", "ntk", "by_parts"):
+        raise ValueError(f"rotary_frequencies: scaling must be none, linear, ntk or by_parts, got {scaling!r}")
+    if scale < 1.0 or (scaling == "none" and scale != 1.0) or not theta > 1.0 or not fast > slow:
+        raise ValueError("rotary_frequencies: needs scale >= 1 (1 without scaling), theta > 1 and fast > slow")
+    i = torch.arange(0, dim, 2, dtype=torch.float64) / dim
+    freqs, factor = theta ** -i, 1.0
+    if scaling == "linear":
+        freqs = freqs / scale
+    elif scaling == "ntk" and dim > 2:
+        freqs = (theta * scale ** (dim / (dim - 2))) ** -i
+    elif scaling == "by_parts":
+        turns = trained * freqs / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        freqs = freqs * keep + freqs / scale * (1 - keep)
+        factor = 0.1 * math.log(scale) + 1.0
+    return freqs.to(device), factor
 
 
 def cos_sin(*tables: torch.Tensor, device) -> tuple[torch.Tensor, torch.Tensor]:

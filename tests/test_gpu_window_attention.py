@@ -1,0 +1,255 @@
+"""``window_attention`` against FP64: windows, first visible keys, ragged lengths, masks, grouped heads,
+strides, long caches, empty rows and non-finite values in places that a query does not see."""
+
+import pytest
+import torch
+
+from iris_mi355x import kernels as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+
+
+def visible(batch, nq, nk, window, sinks, causal, lengths, starts, key_mask):
+    j = torch.arange(nk, device=DEV)
+    length = torch.full((batch,), nk, device=DEV) if lengths is None else lengths.long().clamp(0, nk)
+    if starts is None:
+        start = length - nq
+    else:
+        start = starts.long() if isinstance(starts, torch.Tensor) else torch.full((batch,), starts, device=DEV)
+    p = start[:, None, None] + torch.arange(nq, device=DEV)[:, None]
+    seen = (j < length[:, None, None]).expand(batch, nq, nk)
+    if causal:
+        seen = seen & (j <= p)
+    if window is not None:
+        seen = seen & (((p - j).abs() < window) | (j < sinks))
+    if key_mask is not None:
+        seen = seen & (key_mask != 0)[:, None, :]
+    return seen
+
+
+def reference(q, k, v, window=None, sinks=0, causal=True, lengths=None, starts=None, key_mask=None, scale=None):
+    """``(o, tolerance)`` in FP64, ``[B, Nq, H, 128]``.
+
+    The kernel's scores are FP32 sums of 128 exact products (128 2^-24 of their absolute sum at worst), its
+    weights carry the exponential's and the sum's FP32 errors (n_k 2^-24 at worst) and are rounded to BF16
+    (half a step, 2^-8) before the product with v; the result is rounded to BF16 once more."""
+    group = q.shape[1] // k.shape[1]
+    scale = 128 ** -0.5 if scale is None else scale
+    seen = visible(q.shape[0], q.shape[2], k.shape[2], window, sinks, causal, lengths, starts, key_mask)[:, None]
+    kd, vd = (t.double().repeat_interleave(group, 1) for t in (k, v))
+    # hidden places count for nothing, whatever they hold
+    some = seen.any(2)[:, :, :, None]
+    kd, vd = torch.where(some, kd, 0.0), torch.where(some, vd, 0.0)
+    s = (q.double() @ kd.transpose(-1, -2) * scale).masked_fill(~seen, -torch.inf)
+    off = (q.double().abs() @ kd.abs().transpose(-1, -2) * abs(scale) * 128 * 2.0 ** -24).masked_fill(~seen, 0.0).amax(-1, True)
+    w = torch.where(seen.any(-1, True), torch.softmax(s, -1), 0.0)
+    o, a = w @ vd, w @ vd.abs()
+    tol = (2.0 ** -8 + 2 * off + (k.shape[2] + 16) * 2.0 ** -24) * a + 2.0 ** -8 * o.abs() * 1.01 + 1e-30
+    return o.transpose(1, 2), tol.transpose(1, 2)
+
+
+def check(q, k, v, got=None, **options):
+    if got is None:
+        got = K.window_attention(q, k, v, **options)
+    options.pop("out", None)
+    want, tol = reference(q, k, v, **options)
+    assert got.shape == (q.shape[0], q.shape[2], q.shape[1] * 128) and got.dtype == BF16
+    err = (got.unflatten(-1, (-1, 128)).double() - want).abs()
+    assert (err <= tol).all(), f"worst {(err / tol.clamp(min=1e-30)).max().item():.3g} of the tolerance"
+
+
+def heads_of(seed, batch, nq, nk, heads, kv, gain=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q = gain * torch.randn(batch, heads, nq, 128, generator=g, device=DEV)
+    k, v = (torch.randn(batch, kv, nk, 128, generator=g, device=DEV) for _ in range(2))
+    return q.to(BF16), k.to(BF16), v.to(BF16)
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 33, 64, 65, 127, 128, 200, 300, 513])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (7, 1), (64, 4), (100, 70), (128, 0), (1000, 3)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts(n, window, sinks, causal):
+    q, k, v = heads_of(20, 2, n, n, 4, 1, gain=2.0)
+    check(q, k, v, window=window, sinks=sinks, causal=causal)
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (2, 2), (6, 2), (5, 1), (20, 5), (8, 1), (21, 3), (16, 1), (32, 1)])
+@pytest.mark.parametrize("nq,nk", [(1, 77), (3, 1000), (150, 150), (17, 400)])
+def test_grouped_heads(heads, kv, nq, nk):
+    q, k, v = heads_of(21, 2, nq, nk, heads, kv)
+    check(q, k, v, window=50, sinks=3)
+    check(q, k, v)
+
+
+@pytest.mark.parametrize("nq", [1, 2, 4, 5, 16, 33])
+@pytest.mark.parametrize("nk", [40, 64, 1000, 4097])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (256, 4), (1, 0), (3000, 130)])
+def test_few_queries_over_a_cache(nq, nk, window, sinks):
+    q, k, v = heads_of(22, 3, nq, nk, 20, 5)
+    lengths = torch.tensor([nk, max(nq, nk // 2), min(nq, nk)], device=DEV, dtype=torch.int32)
+    check(q, k, v, window=window, sinks=sinks)
+    check(q, k, v, window=window, sinks=sinks, lengths=lengths)
+    check(q, k, v, window=window, sinks=sinks, lengths=lengths.long(), causal=False)
+
+
+@pytest.mark.parametrize("nk", [16385, 40000])
+@pytest.mark.parametrize("batch", [1, 7])
+def test_long_caches(nk, batch):
+    q, k, v = heads_of(23, batch, 1, nk, 8, 2, gain=3.0)
+    lengths = torch.arange(batch, device=DEV) * (nk // 9) + nk // 3
+    check(q, k, v)
+    check(q, k, v, lengths=lengths)
+    check(q, k, v, lengths=lengths, window=nk // 2, sinks=100)
+
+
+def test_one_query_of_a_peaked_row():
+    """One key far above the others, in the last place, the first, and beside the window's edge."""
+    for at in (0, 1, 499, 500, 998, 999):
+        q, k, v = heads_of(24, 1, 1, 1000, 4, 1)
+        k[0, 0, at] = 4 * q[0, 0, 0]
+        check(q, k, v)
+        check(q, k, v, window=500, sinks=1)
+
+
+@pytest.mark.parametrize("nq,nk", [(1, 300), (120, 120), (130, 700)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("kind", [torch.bool, torch.uint8])
+def test_key_masks(nq, nk, causal, kind):
+    q, k, v = heads_of(25, 4, nq, nk, 4, 2)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    mask = (torch.rand(4, nk, generator=g, device=DEV) < 0.6)
+    mask[1, : nk // 2] = False  # padding in front
+    mask[2] = False  # nothing at all
+    mask = mask.to(kind) * (3 if kind == torch.uint8 else 1)
+    mask = mask.to(kind)
+    for window, sinks in ((None, 0), (20, 2), (90, 0)):
+        out = torch.full((4, nq, 512), 7.0, device=DEV, dtype=BF16)
+        got = K.window_attention(q, k, v, window, sinks, causal=causal, key_mask=mask, out=out)
+        assert got is out and not got[2].any()
+        check(q, k, v, got, window=window, sinks=sinks, causal=causal, key_mask=mask)
+
+
+@pytest.mark.parametrize("starts", [0, 5, -3, 1000, 10**12, "ints"])
+@pytest.mark.parametrize("nq,nk", [(1, 64), (40, 200), (200, 200)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_starts(starts, nq, nk, causal):
+    """Right-padded prompts (starts 0, lengths below Nq), queries before the first key and far past the last."""
+    q, k, v = heads_of(26, 3, nq, nk, 4, 2)
+    if starts == "ints":
+        starts = torch.tensor([0, nk // 2, -nq], device=DEV)
+    lengths = torch.tensor([nk, nk // 3, 0], device=DEV)
+    for window, sinks in ((None, 0), (33, 2), (2 * 10**12, 0)):
+        check(q, k, v, window=window, sinks=sinks, causal=causal, lengths=lengths, starts=starts)
+
+
+def test_lengths_are_clamped():
+    q, k, v = heads_of(27, 3, 2, 50, 2, 1)
+    lengths = torch.tensor([-4, 60, 2**40], device=DEV)
+    got = K.window_attention(q, k, v, lengths=lengths)
+    assert not got[0].any()
+    check(q, k, v, got, lengths=lengths)
+
+
+@pytest.mark.parametrize("nq,nk", [(1, 500), (130, 130)])
+def test_strided_views(nq, nk):
+    """Token-major and packed views, an expanded batch of keys, an output with room between rows."""
+    g = torch.Generator(device=DEV).manual_seed(28)
+    q = torch.randn(3, nq, 8, 136, generator=g, device=DEV).to(BF16)[..., :128].transpose(1, 2)
+    packed = torch.randn(1, nk, 5, 128, generator=g, device=DEV).to(BF16)
+    k, v = packed[:, :, 0:2].transpose(1, 2).expand(3, -1, -1, -1), packed[:, :, 3:5].transpose(1, 2).expand(3, -1, -1, -1)
+    store = torch.full((3, nq + 2, 1100), 7.0, device=DEV, dtype=BF16)
+    out = store[:, 1:-1, 4:1028]
+    K.window_attention(q, k, v, 60, 2, out=out)
+    check(q, k, v, out, window=60, sinks=2)
+    store[:, 1:-1, 4:1028] = 7.0
+    assert (store == 7.0).all()
+
+
+def test_offsets_past_32_bits():
+    rows, stride = 40, 1 << 26
+    flat = torch.empty(rows * stride, device=DEV, dtype=BF16)
+    k = flat.as_strided((1, 1, rows, 128), (rows * stride, 128, stride, 1))
+    v = flat.as_strided((1, 1, rows, 128), (rows * stride, 128, stride, 1), 256)
+    g = torch.Generator(device=DEV).manual_seed(29)
+    k.copy_(torch.randn(rows, 128, generator=g, device=DEV))
+    v.copy_(torch.randn(rows, 128, generator=g, device=DEV))
+    for nq in (1, 40):
+        q = torch.randn(1, 4, nq, 128, generator=g, device=DEV).to(BF16)
+        got = K.window_attention(q, k, v, 30, 2)
+        check(q, k.contiguous(), v.contiguous(), got, window=30, sinks=2)
+
+
+@pytest.mark.parametrize("nq,nk,causal", [(1, 400, True), (3, 400, True), (200, 200, True), (200, 200, False)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_non_finite_values_in_hidden_places(nq, nk, causal, value):
+    """Masked keys, keys past the length and keys outside every query's window hold NaN or infinities; and one
+    key that later queries see does: the rows before it, and after its window, are as if it were not there."""
+    q, k, v = heads_of(30, 2, nq, nk, 4, 2)
+    mask = torch.ones(2, nk, device=DEV, dtype=torch.bool)
+    mask[0, 5:9], mask[1, nk - 40: nk - 35] = False, False
+    lengths = torch.tensor([nk, nk - 3], device=DEV)
+    for window, sinks in ((None, 0), (60, 2)):
+        seen = visible(2, nq, nk, window, sinks, causal, lengths, None, mask)
+        kb, vb = k.clone(), v.clone()
+        hidden = ~seen.any(1)[:, None, :, None]
+        kb.masked_fill_(hidden, value), vb.masked_fill_(hidden, value)
+        options = dict(window=window, sinks=sinks, causal=causal, key_mask=mask, lengths=lengths)
+        got = K.window_attention(q, kb, vb, **options)
+        check(q, k, v, got, **options)
+        at = nk - 30
+        kb, vb = k.clone(), v.clone()
+        vb[:, :, at, 3] = value
+        got = K.window_attention(q, kb, vb, **options).unflatten(-1, (-1, 128))
+        touched = torch.zeros_like(got, dtype=torch.bool)
+        touched[..., 3] = seen[:, :, at, None]
+        assert not torch.isfinite(got[touched]).any()
+        want, tol = reference(q, k, v, **options)
+        assert ((got.double() - want).abs() <= tol)[~touched].all()
+        kb[:, :, at, 7], vb = value, v
+        got = K.window_attention(q, kb, vb, **options).unflatten(-1, (-1, 128))
+        assert ((got.double() - want).abs() <= tol)[~seen[:, :, at]].all()
+
+
+def test_rows_do_not_depend_on_the_batch():
+    q, k, v = heads_of(31, 4, 1, 5000, 8, 2)
+    whole = K.window_attention(q, k, v, 2000, 4)
+    for b in range(4):
+        one = K.window_attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], 2000, 4)
+        assert torch.allclose(one.double(), whole[b:b + 1].double(), rtol=2.0 ** -7, atol=2.0 ** -8)
+    assert torch.equal(whole, K.window_attention(q, k, v, 2000, 4))  # and not on the run
+
+
+def test_empty_calls():
+    for batch, nq, nk in ((0, 3, 5), (2, 0, 5), (2, 3, 0)):
+        q, k, v = heads_of(32, batch, nq, nk, 2, 1)
+        got = K.window_attention(q, k, v, 4, 1)
+        assert got.shape == (batch, nq, 256) and not got.any()
+
+
+def test_streams_and_graphs():
+    """Two captured graphs of split calls replayed in turns, on another stream, with eager calls between."""
+    q, k, v = heads_of(33, 2, 1, 9000, 8, 2)
+    outs = [torch.empty(2, 1, 1024, device=DEV, dtype=BF16) for _ in range(2)]
+    lengths = torch.tensor([9000, 9000], device=DEV)
+    options = [dict(lengths=lengths), dict(lengths=lengths, window=3000, sinks=4)]
+    K.window_attention(q, k, v, out=outs[0], **options[0])
+    torch.cuda.synchronize()
+    graphs = []
+    for out, opt in zip(outs, options):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            K.window_attention(q, k, v, out=out, **opt)
+        graphs.append(graph)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    side = torch.cuda.Stream()
+    for step in range(3):
+        q.normal_(generator=g)
+        lengths.copy_(torch.tensor([9000 - 700 * step, 17 + step]))
+        for graph, out, opt in zip(graphs, outs, options):
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+            torch.cuda.current_stream().wait_stream(side)
+            assert torch.equal(out, K.window_attention(q, k, v, **opt))
