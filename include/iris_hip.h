@@ -32,8 +32,6 @@ enum { IRIS_EPI_NONE = 0, IRIS_EPI_SILU_MUL = 1, IRIS_EPI_SILU = 2 };
 enum { IRIS_ACT_NONE = 0, IRIS_ACT_SILU = 1 };
 /* Rotary pair layouts: elements (i, i + pairs) or (2 i, 2 i + 1). */
 enum { IRIS_ROTARY_HALF = 0, IRIS_ROTARY_INTERLEAVED = 1 };
-/* Per-tensor flags of iris_rotary. */
-enum { IRIS_ROTARY_TURN = 1, IRIS_ROTARY_TO_ROWS = 2 };
 
 const char* iris_last_error(void);
 /* Library ABI version (bumped on any signature change). */
@@ -99,18 +97,31 @@ int iris_qk_norm_rope(const void* src, int src_dtype, void* dst, int dst_dtype, 
                       hipStream_t stream);
 
 /* Rotary positions of up to three tensors of one dtype (query, key and value heads of a projection), no
- * counterpart in the reference: heads of x[i] (strides of batch item, token and head in x_strides[3 i ..],
- * elements; unit stride inside a head) go to out[i] (strides of batch item, head and row). With
- * IRIS_ROTARY_TURN in flags[i], pair j < pairs of token t turns by positions[b, t] freqs[j] (formed in FP64) in
- * the given layout, scaled by `factor`, the other elements are copied; without it all are. transpose: turns by
- * the negative angle (the gradient). Token t goes to row t, with IRIS_ROTARY_TO_ROWS to row rows[b, t], and
- * nowhere if that lies outside [0, out_rows[i]). positions / rows: int32 (kind 1) or int64 (kind 3), batch rows
- * `*_stride` apart (0: shared). out[i] may be x[i] itself, element for element, without TO_ROWS. */
-int iris_rotary(int tensors, const void* const* x, const long* x_strides, void* const* out, const long* out_strides,
-                const int* heads, const int* flags, const long* out_rows, int dtype, int batch, long tokens,
-                int head_dim, const void* positions, int positions_kind, long positions_stride, const void* rows,
-                int rows_kind, long rows_stride, const double* freqs, int pairs, int layout, float factor,
-                int transpose, hipStream_t stream);
+ * counterpart in the reference: heads t[i].x [batch, tokens, heads, head_dim] go to t[i].out [batch, heads, rows,
+ * head_dim] (any strides, in elements; unit stride inside a head). In the first `turned` tensors pair j < pairs of
+ * token n turns by positions[b, n] freqs[j] (formed in FP64) in the given layout, scaled by `factor`, and the
+ * other elements are copied; in the rest all are. transpose: turns by the negative angle (the gradient). Token n
+ * goes to row n, in the tensors from `to_rows` on to row rows[b, n], and nowhere if that row does not exist.
+ * positions / rows: int32 (kind 1) or int64 (kind 3), batch rows `*_stride` apart (0: shared). out may be x
+ * itself, element for element, before `to_rows`; else the two must lie apart. */
+typedef struct {
+  const void* x;
+  long x_shape[4], x_strides[4];
+  void* out;
+  long out_shape[4], out_strides[4];
+} iris_rotary_tensor;
+typedef struct {
+  long tensors, turned, to_rows, dtype;
+  iris_rotary_tensor t[3];
+  const void* positions;
+  long positions_kind, positions_stride;
+  const void* rows;
+  long rows_kind, rows_stride;
+  const double* freqs;
+  long pairs, layout, transpose;
+  double factor;
+} iris_rotary_args;
+int iris_rotary(const iris_rotary_args* args, hipStream_t stream);
 
 /* The V half of the attention input (src/iris_metal/model.py:243-250 builds [B,Hkv,N,128]):
  * heads at col_offset of a BF16 [batch, n_src, row_stride] projection are written transposed
@@ -174,17 +185,32 @@ int iris_flash_attn_masked(const void* q, const void* k, const void* vt, int bat
 
 /* Attention with a sliding window and a few first keys that stay visible (no counterpart in the reference):
  * softmax(q k^T * scale) v of BF16 heads of 128, q [batch, heads, n_q, 128], k and v [batch, kv_heads, n_k, 128]
- * by their strides of batch item, head and row (elements, multiples of 8; 16-byte aligned). Query t of item b is
- * at position start_b + t and sees key j < length_b where (not causal or j <= position) and (window == 0 or
+ * (any strides that are multiples of 8 elements, unit stride inside a head; 16-byte aligned). Query t of item b
+ * is at position start_b + t and sees key j < length_b where (not causal or j <= position) and (window == 0 or
  * |position - j| < window or j < sinks) and (key_mask null or key_mask[b * mask_stride + j] != 0); a row that
  * sees nothing is 0. lengths: null (n_k) or [batch], clamped to [0, n_k]; starts: [batch] of kind 1 or 3, the
- * value `start` (kind 4), or length_b - n_q (kind 0). Integer kinds: 1 int32, 3 int64. out BF16: row t of item b
- * at b out_strides[0] + t out_strides[1], column h * 128 + d. K and V of keys that no query sees are not used. */
-int iris_window_attn(const void* q, const long* q_strides, const void* k, const long* k_strides, const void* v,
-                     const long* v_strides, void* out, const long* out_strides, int batch, int heads, int kv_heads,
-                     long n_q, long n_k, long window, long sinks, int causal, const void* lengths, int lengths_kind,
-                     const void* starts, int starts_kind, long start, const void* key_mask, long mask_stride,
-                     float scale, hipStream_t stream);
+ * value `start` (kind 4), or length_b - n_q (kind 0). Integer kinds: 1 int32, 3 int64. out BF16 [batch, n_q,
+ * heads * 128], unit column stride, other strides multiples of 4. K and V of keys that no query sees are not
+ * used. workspace: iris_window_attn_workspace(args) bytes, 16-byte aligned (null if that is 0); its contents
+ * matter to no other call. */
+typedef struct {
+  const void *q, *k, *v;
+  void* out;
+  long q_shape[4], q_strides[4], k_shape[4], k_strides[4], v_shape[4], v_strides[4], out_shape[3], out_strides[3];
+  long window, sinks, causal;
+  const void* lengths;
+  long lengths_kind;
+  const void* starts;
+  long starts_kind, start;
+  const void* key_mask;
+  long mask_stride;
+  double scale;
+  void* workspace;
+  long workspace_bytes;
+} iris_window_attn_args;
+int iris_window_attn(const iris_window_attn_args* args, hipStream_t stream);
+/* Bytes of workspace that iris_window_attn needs for these arguments (by shapes, window, sinks and causal alone). */
+int iris_window_attn_workspace(const iris_window_attn_args* args, long* bytes);
 
 /* mask.bool() of the encoder's [batch, >= n] attention mask (row stride ld elements) as the
  * [batch, n_pad] 0/1 bytes iris_flash_attn_masked reads (src/iris3b/nn/embeddings.py:199);
@@ -296,10 +322,18 @@ int iris_timestep_gemv_bf16(const float* t, const float* freqs, int half, const 
  * scales FP32 or BF16 [n, ceil(k / group)]. y[b, n] = act_out(sum_k W[n, k] act_in(x[b, k]) + bias[n]) with FP32
  * sums and x FP32 or BF16 [batch, k]; out FP32 or BF16 [batch, n], or with n_extra > 0 [n_extra, batch, n]:
  * out[j, b, n] = y[b, n] + extra_bias[j, n]. k and group multiples of 32, codes and x 16-byte aligned. */
-int iris_gemv_w4(int jobs, const void* const* codes, const void* const* scales, int scales_dtype,
-                 const void* const* zeros, int group, const void* x, int x_dtype, int batch, const int* n, int k,
-                 const float* const* bias, const float* const* extra_bias, const int* n_extra, void* const* out,
-                 int out_dtype, int in_act, int out_act, hipStream_t stream);
+typedef struct {
+  const void *codes, *scales, *zeros;
+  const float *bias, *extra_bias;
+  void* out;
+  long n, n_extra;
+} iris_gemv_w4_job;
+typedef struct {
+  long jobs, batch, k, group, x_dtype, out_dtype, scales_dtype, in_act, out_act;
+  const void* x;
+  iris_gemv_w4_job job[2];
+} iris_gemv_w4_args;
+int iris_gemv_w4(const iris_gemv_w4_args* args, hipStream_t stream);
 
 /* Sinusoidal timestep features [cos | sin] (src/iris3b/nn/embeddings.py:41-45):
  * out[b, j] = cos(t[b] * freqs[j]), out[b, half + j] = sin(t[b] * freqs[j]). */

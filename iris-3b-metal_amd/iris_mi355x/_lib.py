@@ -8,6 +8,7 @@ tensors. There is no fallback: if the library is missing, or no GPU is present, 
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_float, c_int, c_long, c_void_p
 from pathlib import Path
 
@@ -20,7 +21,6 @@ F32, BF16 = 0, 1
 EPI_NONE, EPI_SILU_MUL, EPI_SILU = 0, 1, 2
 ACT_NONE, ACT_SILU = 0, 1
 ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
-ROTARY_TURN, ROTARY_TO_ROWS = 1, 2
 E_INVALID, E_LAUNCH, E_UNSUPPORTED = -1, -2, -3
 
 P = c_void_p
@@ -44,11 +44,10 @@ _SIGNATURES: dict[str, list] = {
     "iris_gemm_force_tile": [c_int],
     "iris_flash_attn_force_variant": [c_int],
     "iris_flash_attn_masked": [P, P, P, c_int, c_int, c_int, c_long, c_long, c_float, P, P, c_long, c_long, P],
-    "iris_rotary": [c_int, P, P, P, P, P, P, P, c_int, c_int, c_long, c_int, P, c_int, c_long, P, c_int, c_long, P, c_int,
-                    c_int, c_float, c_int, P],
-    "iris_window_attn": [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_long, c_long, c_long, c_long, c_int, P, c_int, P,
-                         c_int, c_long, P, c_long, c_float, P],
-    "iris_gemv_w4": [c_int, P, P, c_int, P, c_int, P, c_int, c_int, P, c_int, P, P, P, P, c_int, c_int, c_int, P],
+    "iris_rotary": [P, P],
+    "iris_window_attn": [P, P],
+    "iris_window_attn_workspace": [P, P],
+    "iris_gemv_w4": [P, P],
     "iris_text_key_mask": [P, c_int, c_long, c_int, c_long, c_long, P, P],
     "iris_layer_attention": [P, P, c_long, c_int, c_int, c_int, c_float, P],
     "iris_layer_pool": [P, P, P, P, c_long, c_int, c_int, P, c_int, P],
@@ -75,6 +74,12 @@ _SIGNATURES: dict[str, list] = {
     "iris_cfg_combine": [P, P, c_long, c_float, P, P],
     "iris_clamp": [P, c_long, c_float, c_float, P, P],
 }
+
+# Argument structs of the entry points that take one: all fields 8 bytes wide (pointers and integers "q", FP64 "d"),
+# in the header's order. struct.pack of a whole struct costs less than ten ctypes conversions.
+ROTARY_ARGS = struct.Struct("=4q" + 3 * "18q" + "10qd")
+WINDOW_ATTN_ARGS = struct.Struct("=4q24q6q3q2q3q2qd2q")
+GEMV_W4_ARGS = struct.Struct("=9qq" + 2 * "8q")
 
 _lib: ctypes.CDLL | None = None
 

@@ -9,6 +9,12 @@
 // The angle is formed in 64 bits and reduced to a fraction of a turn there: at position 2^20 an FP32
 // product is already 0.06 radians off. cos and sin of the reduced turn are FP32, the rotation FP32 with
 // one rounding to the output type.
+//
+// Bound by memory: every element is read and written once. A workgroup takes `tok` tokens of one item,
+// computes their (cos, sin) into LDS once for all heads of all tensors, then moves the heads in chunks
+// of 16 bytes (both halves of a pair chunk in one thread, so that a rotation in place is safe);
+// consecutive threads take consecutive chunks of a head, then the next head of the token. Odd widths and
+// strides, and unaligned tensors, go element by element through the same code.
 #include "iris_common.hpp"
 
 namespace iris {
@@ -29,6 +35,7 @@ struct RotaryArgs {
   RotaryTensor t[kMaxTensors];
   int tensors, heads_total;
   long tokens;
+  int tok;  // tokens per workgroup
   int head_dim, pairs, interleaved;
   const void* positions;
   const void* rows;
@@ -49,39 +56,116 @@ __device__ __forceinline__ void turn_of(double p, double f, float& c, float& s) 
   sincospif(static_cast<float>(2.0 * turn), &s, &c);
 }
 
-// One workgroup per (token, batch item); a thread per pair (or pair of copied elements).
-template <typename T>
+template <typename T, int N>
+struct Chunk {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Chunk<T, N> load_chunk(const T* p) {
+  Chunk<T, N> c;
+  if constexpr (N * sizeof(T) == 16) {
+    *reinterpret_cast<int4*>(&c) = *reinterpret_cast<const int4*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) c.v[i] = p[i];
+  }
+  return c;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_chunk(T* p, const Chunk<T, N>& c) {
+  if constexpr (N * sizeof(T) == 16) {
+    *reinterpret_cast<int4*>(p) = *reinterpret_cast<const int4*>(&c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = c.v[i];
+  }
+}
+
+// VEC: elements per chunk (16 bytes, or 1: half layout, 2: interleaved, by single elements).
+template <typename T, int VEC, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-  const long n = blockIdx.x;
+  extern __shared__ f32x2 turns[];  // [tok][pairs] (cos, sin)
+  const long n0 = static_cast<long>(blockIdx.x) * a.tok;
   const int b = blockIdx.y;
-  const double p = static_cast<double>(index_at(a.positions, a.positions64, b * a.positions_stride + n));
-  const int half = a.head_dim / 2;
-  for (int i = threadIdx.x; i < a.heads_total * half; i += blockDim.x) {
-    int h = i / half;
-    const int pair = i - h * half;
-    int j = 0;
-    while (h >= a.t[j].heads) h -= a.t[j++].heads;
-    const RotaryTensor& t = a.t[j];
-    const long row = (t.flags & kToRows) ? index_at(a.rows, a.rows64, b * a.rows_stride + n) : n;
-    if (row < 0 || row >= t.out_rows) continue;
-    const bool turned = (t.flags & kTurn) && pair < a.pairs;
-    const int e0 = turned && !a.interleaved ? pair : 2 * pair;
-    const int e1 = turned && !a.interleaved ? pair + a.pairs : 2 * pair + 1;
-    const T* x = static_cast<const T*>(t.x) + b * t.xs_b + n * t.xs_n + h * t.xs_h;
-    T* y = static_cast<T*>(t.out) + b * t.os_b + h * t.os_h + row * t.os_n;
-    const T x0 = x[e0], x1 = x[e1];
-    if (!turned) {
-      y[e0] = x0;
-      y[e1] = x1;
-      continue;
-    }
+  const int ntok = static_cast<int>(a.tokens - n0 < a.tok ? a.tokens - n0 : a.tok);
+  for (int i = threadIdx.x; i < ntok * a.pairs; i += 256) {
+    const int t = i / a.pairs, pair = i - t * a.pairs;
+    const double p = static_cast<double>(index_at(a.positions, a.positions64, b * a.positions_stride + n0 + t));
     float c, s;
     turn_of(p, a.freqs[pair], c, s);
-    c *= a.factor;
-    s *= a.factor * a.sign;
-    const float f0 = to_f32(x0), f1 = to_f32(x1);
-    y[e0] = from_f32<T>(__builtin_fmaf(f0, c, -(f1 * s)));
-    y[e1] = from_f32<T>(__builtin_fmaf(f1, c, f0 * s));
+    turns[i] = f32x2{c * a.factor, s * a.factor * a.sign};
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int j = 0; j < a.tensors; ++j) {
+    const RotaryTensor& t = a.t[j];
+    const int turned = (t.flags & kTurn) ? a.pairs : 0;
+    // items of a head: rotated ones (two chunks in the half layout, one in the interleaved), then copied chunks
+    const int turning = INTERLEAVED ? 2 * turned / VEC : turned / VEC;
+    const int items = turning + (a.head_dim - 2 * turned) / VEC;
+    const int lanes = items < 256 ? items : 256;
+    const int slots = 256 / lanes;
+    const int slot = threadIdx.x / lanes, c0 = threadIdx.x - slot * lanes;
+    if (slot >= slots) continue;
+    int tok = slot / t.heads, h = slot - tok * t.heads;
+    while (tok < ntok) {
+      const long n = n0 + tok;
+      const long row = (t.flags & kToRows) ? index_at(a.rows, a.rows64, b * a.rows_stride + n) : n;
+      if (row >= 0 && row < t.out_rows) {
+        const T* x = static_cast<const T*>(t.x) + b * t.xs_b + n * t.xs_n + h * t.xs_h;
+        T* y = static_cast<T*>(t.out) + b * t.os_b + h * t.os_h + row * t.os_n;
+        for (int c = c0; c < items; c += lanes) {
+          if (c >= turning) {
+            const int e = 2 * turned + (c - turning) * VEC;
+            store_chunk<T, VEC>(y + e, load_chunk<T, VEC>(x + e));
+          } else if constexpr (INTERLEAVED) {
+            const int e = c * VEC;
+            const f32x2* cs = turns + tok * a.pairs + e / 2;
+            Chunk<T, VEC> v = load_chunk<T, VEC>(x + e);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+              const float x0 = to_f32(v.v[2 * i]), x1 = to_f32(v.v[2 * i + 1]);
+              const f32x2 r = cs[i];
+              v.v[2 * i] = from_f32<T>(__builtin_fmaf(x0, r[0], -(x1 * r[1])));
+              v.v[2 * i + 1] = from_f32<T>(__builtin_fmaf(x1, r[0], x0 * r[1]));
+            }
+            store_chunk<T, VEC>(y + e, v);
+          } else {
+            const int e = c * VEC;
+            const f32x2* cs = turns + tok * a.pairs + e;
+            Chunk<T, VEC> u = load_chunk<T, VEC>(x + e), v = load_chunk<T, VEC>(x + e + turned);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const float x0 = to_f32(u.v[i]), x1 = to_f32(v.v[i]);
+              const f32x2 r = cs[i];
+              u.v[i] = from_f32<T>(__builtin_fmaf(x0, r[0], -(x1 * r[1])));
+              v.v[i] = from_f32<T>(__builtin_fmaf(x1, r[0], x0 * r[1]));
+            }
+            store_chunk<T, VEC>(y + e, u);
+            store_chunk<T, VEC>(y + e + turned, v);
+          }
+        }
+      }
+      for (h += slots; h >= t.heads; h -= t.heads) ++tok;
+    }
+  }
+}
+
+template <typename T>
+void launch_rotary(const RotaryArgs& a, bool vector, int batch, hipStream_t stream) {
+  constexpr int kVec = 16 / sizeof(T);
+  const dim3 grid(static_cast<unsigned>((a.tokens + a.tok - 1) / a.tok), batch);
+  const size_t lds = static_cast<size_t>(a.tok) * a.pairs * sizeof(f32x2);
+  if (a.interleaved) {
+    if (vector)
+      rotary_kernel<T, kVec, true><<<grid, 256, lds, stream>>>(a);
+    else
+      rotary_kernel<T, 2, true><<<grid, 256, lds, stream>>>(a);
+  } else {
+    if (vector)
+      rotary_kernel<T, kVec, false><<<grid, 256, lds, stream>>>(a);
+    else
+      rotary_kernel<T, 1, false><<<grid, 256, lds, stream>>>(a);
   }
 }
 
@@ -90,61 +174,96 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 
 using namespace iris;
 
-extern "C" int iris_rotary(int tensors, const void* const* x, const long* x_strides, void* const* out,
-                           const long* out_strides, const int* heads, const int* flags, const long* out_rows,
-                           int dtype, int batch, long tokens, int head_dim, const void* positions,
-                           int positions_kind, long positions_stride, const void* rows, int rows_kind,
-                           long rows_stride, const double* freqs, int pairs, int layout, float factor, int transpose,
-                           hipStream_t stream) {
-  IRIS_REQUIRE(tensors >= 1 && tensors <= kMaxTensors && x && x_strides && out && out_strides && heads && flags &&
-                   out_rows,
+namespace {
+// First and one-past-last address of a tensor.
+void extent(const void* p, const long* shape, const long* strides, int dims, int size, uintptr_t* lo, uintptr_t* hi) {
+  long first = 0, last = 0;
+  for (int i = 0; i < dims; ++i) (strides[i] < 0 ? first : last) += (shape[i] - 1) * strides[i];
+  *lo = reinterpret_cast<uintptr_t>(p) + first * size;
+  *hi = reinterpret_cast<uintptr_t>(p) + (last + 1) * size;
+}
+}  // namespace
+
+extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
+  IRIS_REQUIRE(args, "rotary: null pointer");
+  const iris_rotary_args& g = *args;
+  IRIS_REQUIRE(g.tensors >= 1 && g.tensors <= kMaxTensors && g.turned >= 0 && g.to_rows >= 0,
                "rotary: takes one to three tensors");
-  IRIS_REQUIRE(dtype == IRIS_F32 || dtype == IRIS_BF16, "rotary: unknown dtype %d", dtype);
+  IRIS_REQUIRE(g.dtype == IRIS_F32 || g.dtype == IRIS_BF16, "rotary: unknown dtype %ld", g.dtype);
+  const long batch = g.t[0].x_shape[0], tokens = g.t[0].x_shape[1], dim = g.t[0].x_shape[3];
   IRIS_REQUIRE(batch >= 0 && batch < 65536 && tokens >= 0 && tokens < (1L << 31), "rotary: bad batch or token count");
-  IRIS_REQUIRE(head_dim > 0 && head_dim % 2 == 0 && head_dim <= 1024 && pairs > 0 && 2 * pairs <= head_dim,
-               "rotary: need an even head width up to 1024 that holds the %d rotated pairs (got %d)", pairs, head_dim);
-  IRIS_REQUIRE(layout == IRIS_ROTARY_HALF || layout == IRIS_ROTARY_INTERLEAVED, "rotary: unknown layout %d", layout);
-  if (batch == 0 || tokens == 0) return IRIS_OK;
-  IRIS_REQUIRE(positions && freqs, "rotary: null pointer");
-  IRIS_REQUIRE(positions_kind == 1 || positions_kind == 3, "rotary: positions are int32 (1) or int64 (3)");
+  IRIS_REQUIRE(dim > 0 && dim % 2 == 0 && dim <= 1024 && g.pairs > 0 && 2 * g.pairs <= dim,
+               "rotary: need an even head width up to 1024 that holds the %ld rotated pairs (got %ld)", g.pairs, dim);
+  IRIS_REQUIRE(g.layout == IRIS_ROTARY_HALF || g.layout == IRIS_ROTARY_INTERLEAVED, "rotary: unknown layout %ld", g.layout);
+  IRIS_REQUIRE(g.positions_kind == 1 || g.positions_kind == 3, "rotary: positions are int32 (1) or int64 (3)");
+  const int size = g.dtype == IRIS_F32 ? 4 : 2;
   RotaryArgs a{};
-  for (int i = 0; i < tensors; ++i) {
-    IRIS_REQUIRE(x[i] && out[i] && heads[i] > 0 && out_rows[i] >= 0, "rotary: tensor %d: null pointer or bad sizes", i);
-    IRIS_REQUIRE(!(flags[i] & kToRows) || (rows && (rows_kind == 1 || rows_kind == 3)),
-                 "rotary: tensor %d goes to rows, which are missing or neither int32 (1) nor int64 (3)", i);
-    IRIS_REQUIRE((flags[i] & kToRows) || out_rows[i] >= tokens, "rotary: output %d holds fewer rows than tokens", i);
-    a.t[i] = RotaryTensor{x[i],
-                          out[i],
-                          x_strides[3 * i],
-                          x_strides[3 * i + 1],
-                          x_strides[3 * i + 2],
-                          out_strides[3 * i],
-                          out_strides[3 * i + 1],
-                          out_strides[3 * i + 2],
-                          out_rows[i],
-                          heads[i],
-                          flags[i]};
-    a.heads_total += heads[i];
+  for (int i = 0; i < g.tensors; ++i) {
+    const iris_rotary_tensor& t = g.t[i];
+    const long heads = t.x_shape[2], rows = t.out_shape[2];
+    const bool to_rows = i >= g.to_rows;
+    IRIS_REQUIRE(t.x_shape[0] == batch && t.x_shape[1] == tokens && t.x_shape[3] == dim && heads > 0 && heads <= 4096 &&
+                     t.x_strides[3] == 1,
+                 "rotary: tensor %d: heads must be [%ld, %ld, H, %ld] with unit stride in a head", i, batch, tokens, dim);
+    IRIS_REQUIRE(t.out_shape[0] == batch && t.out_shape[1] == heads && t.out_shape[3] == dim && rows >= 0 &&
+                     rows < (1L << 40) && (to_rows || rows == tokens) && t.out_strides[3] == 1,
+                 "rotary: output %d must be [%ld, %ld, %s, %ld] with unit stride in a head", i, batch, heads,
+                 to_rows ? "rows" : "tokens", dim);
+    IRIS_REQUIRE(!to_rows || g.rows_kind == 1 || g.rows_kind == 3, "rotary: rows are int32 (1) or int64 (3)");
+    a.t[i] = RotaryTensor{t.x,
+                          t.out,
+                          t.x_strides[0],
+                          t.x_strides[1],
+                          t.x_strides[2],
+                          t.out_strides[0],
+                          t.out_strides[1],
+                          t.out_strides[2],
+                          rows,
+                          static_cast<int>(heads),
+                          (i < g.turned ? kTurn : 0) | (to_rows ? kToRows : 0)};
+    a.heads_total += static_cast<int>(heads);
+    if (batch == 0 || tokens == 0 || rows == 0) continue;
+    IRIS_REQUIRE(t.x && t.out && g.positions && g.freqs && (!to_rows || g.rows), "rotary: null pointer");
+    IRIS_REQUIRE((batch == 1 || t.out_strides[0]) && (heads == 1 || t.out_strides[1]) && (rows == 1 || t.out_strides[2]),
+                 "rotary: output %d is an expanded tensor", i);
+    uintptr_t x0, x1, y0, y1;
+    extent(t.x, t.x_shape, t.x_strides, 4, size, &x0, &x1);
+    extent(t.out, t.out_shape, t.out_strides, 4, size, &y0, &y1);
+    const bool same = t.x == t.out && !to_rows && t.x_strides[0] == t.out_strides[0] &&
+                      t.x_strides[1] == t.out_strides[2] && t.x_strides[2] == t.out_strides[1];
+    IRIS_REQUIRE(same || x1 <= y0 || y1 <= x0,
+                 "rotary: output %d must be its input itself (as [B, H, N, D]) or lie apart from it", i);
   }
-  IRIS_REQUIRE(a.heads_total <= 65536, "rotary: too many heads");
-  a.tensors = tensors;
+  if (batch == 0 || tokens == 0) return IRIS_OK;
+  a.tensors = static_cast<int>(g.tensors);
   a.tokens = tokens;
-  a.head_dim = head_dim;
-  a.pairs = pairs;
-  a.interleaved = layout == IRIS_ROTARY_INTERLEAVED;
-  a.positions = positions;
-  a.positions64 = positions_kind == 3;
-  a.positions_stride = positions_stride;
-  a.rows = rows;
-  a.rows64 = rows_kind == 3;
-  a.rows_stride = rows_stride;
-  a.freqs = freqs;
-  a.factor = factor;
-  a.sign = transpose ? -1.0f : 1.0f;
-  const dim3 grid(static_cast<unsigned>(tokens), batch);
-  if (dtype == IRIS_F32)
-    rotary_kernel<float><<<grid, 256, 0, stream>>>(a);
+  a.head_dim = static_cast<int>(dim);
+  a.pairs = static_cast<int>(g.pairs);
+  a.interleaved = g.layout == IRIS_ROTARY_INTERLEAVED;
+  a.positions = g.positions;
+  a.positions64 = g.positions_kind == 3;
+  a.positions_stride = g.positions_stride;
+  a.rows = g.rows;
+  a.rows64 = g.rows_kind == 3;
+  a.rows_stride = g.rows_stride;
+  a.freqs = g.freqs;
+  a.factor = static_cast<float>(g.factor);
+  a.sign = g.transpose ? -1.0f : 1.0f;
+  // one token per workgroup while that leaves the CUs short of workgroups, up to eight (as many share one
+  // set of launch and index work; more tokens gain nothing)
+  const long per = batch * tokens / (8 * device_cus());
+  a.tok = static_cast<int>(per < 1 ? 1 : (per > 8 ? 8 : per));
+  // chunks of 16 bytes where every chunk of every head is aligned and whole
+  const long vec = 16 / size;
+  bool vector = (a.interleaved ? 2 * g.pairs : g.pairs) % vec == 0 && (dim - 2 * g.pairs) % vec == 0;
+  for (int i = 0; i < g.tensors; ++i) {
+    const iris_rotary_tensor& t = g.t[i];
+    vector = vector && aligned(t.x, 16) && aligned(t.out, 16);
+    for (int d = 0; d < 3; ++d) vector = vector && t.x_strides[d] % vec == 0 && t.out_strides[d] % vec == 0;
+  }
+  if (g.dtype == IRIS_F32)
+    launch_rotary<float>(a, vector, static_cast<int>(batch), stream);
   else
-    rotary_kernel<bf16><<<grid, 256, 0, stream>>>(a);
+    launch_rotary<bf16>(a, vector, static_cast<int>(batch), stream);
   return check_launch("rotary");
 }

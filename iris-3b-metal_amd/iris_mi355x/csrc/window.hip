@@ -28,7 +28,7 @@ struct WindowArgs {
   float scale_log2;
 };
 
-__device__ __forceinline__ long clamp_long(long x, long lo, long hi) { return x < lo ? lo : (x > hi ? hi : x); }
+__host__ __device__ __forceinline__ long clamp_long(long x, long lo, long hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
 // Keys of item b that exist, and the position of its first query.
 __device__ __forceinline__ int item_length(const WindowArgs& p, int b) {
@@ -99,53 +99,93 @@ __global__ __launch_bounds__(256) void window_rows_kernel(WindowArgs p, long tot
 
 using namespace iris;
 
-extern "C" int iris_window_attn(const void* q, const long* q_strides, const void* k, const long* k_strides,
-                                const void* v, const long* v_strides, void* out, const long* out_strides, int batch,
-                                int heads, int kv_heads, long n_q, long n_k, long window, long sinks, int causal,
-                                const void* lengths, int lengths_kind, const void* starts, int starts_kind, long start,
-                                const void* key_mask, long mask_stride, float scale, hipStream_t stream) {
-  IRIS_REQUIRE(batch >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
-               "window_attn: query heads %d must be a multiple of K/V heads %d", heads, kv_heads);
+namespace {
+void extent(const void* p, const long* shape, const long* strides, int dims, uintptr_t* lo, uintptr_t* hi) {
+  long first = 0, last = 0;
+  for (int i = 0; i < dims; ++i) (strides[i] < 0 ? first : last) += (shape[i] - 1) * strides[i];
+  *lo = reinterpret_cast<uintptr_t>(p) + first * 2;
+  *hi = reinterpret_cast<uintptr_t>(p) + (last + 1) * 2;
+}
+
+// Checks the arguments and turns them into the kernels' form; p.batch stays 0 where there is nothing to do.
+int window_args(const iris_window_attn_args* args, WindowArgs& p) {
+  IRIS_REQUIRE(args, "window_attn: null pointer");
+  const iris_window_attn_args& g = *args;
+  const long batch = g.q_shape[0], heads = g.q_shape[1], n_q = g.q_shape[2], kv_heads = g.k_shape[1], n_k = g.k_shape[2];
+  for (int i = 0; i < 4; ++i)
+    IRIS_REQUIRE(g.k_shape[i] == g.v_shape[i], "window_attn: k and v must be of one shape");
+  IRIS_REQUIRE(batch >= 0 && batch < 65536 && heads > 0 && kv_heads > 0 && heads <= 65536 && heads % kv_heads == 0 &&
+                   g.k_shape[0] == batch && g.q_shape[3] == kHd && g.k_shape[3] == kHd,
+               "window_attn: q [%ld, %ld, %ld, %ld] and k / v [%ld, %ld, %ld, %ld] do not match: one batch, 128-wide heads, "
+               "a multiple of K/V heads",
+               batch, heads, n_q, g.q_shape[3], g.k_shape[0], kv_heads, n_k, g.k_shape[3]);
   IRIS_REQUIRE(n_q >= 0 && n_k >= 0 && n_q < (1L << 30) && n_k < (1L << 30), "window_attn: need fewer than 2^30 rows");
-  IRIS_REQUIRE(window >= 0 && sinks >= 0, "window_attn: window and sinks must not be negative");
-  IRIS_REQUIRE(!lengths || lengths_kind == 1 || lengths_kind == 3, "window_attn: lengths are int32 (1) or int64 (3)");
-  IRIS_REQUIRE(starts_kind == 0 || starts_kind == 4 || ((starts_kind == 1 || starts_kind == 3) && starts),
+  IRIS_REQUIRE(g.window >= 0 && g.sinks >= 0, "window_attn: window and sinks must not be negative");
+  IRIS_REQUIRE(!g.lengths || g.lengths_kind == 1 || g.lengths_kind == 3, "window_attn: lengths are int32 (1) or int64 (3)");
+  IRIS_REQUIRE(g.starts_kind == 0 || g.starts_kind == 4 || ((g.starts_kind == 1 || g.starts_kind == 3) && g.starts),
                "window_attn: starts are int32 (1), int64 (3), one value (4) or absent (0)");
+  IRIS_REQUIRE(g.out_shape[0] == batch && g.out_shape[1] == n_q && g.out_shape[2] == heads * kHd && g.out_strides[2] == 1,
+               "window_attn: out must be [%ld, %ld, %ld] with unit column stride", batch, n_q, heads * kHd);
+  IRIS_REQUIRE(g.q_strides[3] == 1 && g.k_strides[3] == 1 && g.v_strides[3] == 1,
+               "window_attn: heads must have unit stride");
   if (batch == 0 || n_q == 0) return IRIS_OK;
-  IRIS_REQUIRE(q && q_strides && k_strides && v_strides && out && out_strides && (n_k == 0 || (k && v)),
-               "window_attn: null pointer");
-  IRIS_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 8),
+  IRIS_REQUIRE(g.q && g.out && (n_k == 0 || (g.k && g.v)), "window_attn: null pointer");
+  IRIS_REQUIRE(aligned(g.q, 16) && aligned(g.k, 16) && aligned(g.v, 16) && aligned(g.out, 8),
                "window_attn: inputs must be 16-byte aligned, the output 8");
   for (int i = 0; i < 3; ++i)
-    IRIS_REQUIRE(q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0,
+    IRIS_REQUIRE(g.q_strides[i] % 8 == 0 && g.k_strides[i] % 8 == 0 && g.v_strides[i] % 8 == 0,
                  "window_attn: strides must be multiples of 8 elements");
-  IRIS_REQUIRE(out_strides[0] % 4 == 0 && out_strides[1] % 4 == 0, "window_attn: output strides must be multiples of 4");
-  WindowArgs p{};
-  p.q = static_cast<const bf16*>(q);
-  p.k = static_cast<const bf16*>(k);
-  p.v = static_cast<const bf16*>(v);
-  p.out = static_cast<bf16*>(out);
-  p.qs_b = q_strides[0], p.qs_h = q_strides[1], p.qs_n = q_strides[2];
-  p.ks_b = k_strides[0], p.ks_h = k_strides[1], p.ks_n = k_strides[2];
-  p.vs_b = v_strides[0], p.vs_h = v_strides[1], p.vs_n = v_strides[2];
-  p.os_b = out_strides[0], p.os_n = out_strides[1];
-  p.batch = batch;
-  p.heads = heads;
-  p.kv_heads = kv_heads;
+  IRIS_REQUIRE((n_q == 1 || g.out_strides[1] >= heads * kHd) && (batch == 1 || g.out_strides[0] >= heads * kHd) &&
+                   g.out_strides[0] % 4 == 0 && g.out_strides[1] % 4 == 0,
+               "window_attn: output rows must not overlap, strides must be multiples of 4");
+  uintptr_t o0, o1, x0, x1;
+  extent(g.out, g.out_shape, g.out_strides, 3, &o0, &o1);
+  const void* in[3] = {g.q, g.k, g.v};
+  const long* shapes[3] = {g.q_shape, g.k_shape, g.v_shape};
+  const long* strides[3] = {g.q_strides, g.k_strides, g.v_strides};
+  for (int i = 0; i < (n_k ? 3 : 1); ++i) {
+    extent(in[i], shapes[i], strides[i], 4, &x0, &x1);
+    IRIS_REQUIRE(o1 <= x0 || x1 <= o0, "window_attn: out must lie apart from q, k and v");
+  }
+  p.q = static_cast<const bf16*>(g.q);
+  p.k = static_cast<const bf16*>(g.k);
+  p.v = static_cast<const bf16*>(g.v);
+  p.out = static_cast<bf16*>(g.out);
+  p.qs_b = g.q_strides[0], p.qs_h = g.q_strides[1], p.qs_n = g.q_strides[2];
+  p.ks_b = g.k_strides[0], p.ks_h = g.k_strides[1], p.ks_n = g.k_strides[2];
+  p.vs_b = g.v_strides[0], p.vs_h = g.v_strides[1], p.vs_n = g.v_strides[2];
+  p.os_b = g.out_strides[0], p.os_n = g.out_strides[1];
+  p.batch = static_cast<int>(batch);
+  p.heads = static_cast<int>(heads);
+  p.kv_heads = static_cast<int>(kv_heads);
   p.n_q = static_cast<int>(n_q);
   p.n_k = static_cast<int>(n_k);
-  p.window = window < (1L << 60) ? window : (1L << 60);
-  p.sinks = sinks;
-  p.causal = causal;
-  p.lengths = lengths;
-  p.lengths64 = lengths_kind == 3;
-  p.starts = starts;
-  p.starts_kind = starts_kind;
-  p.start = start;
-  p.key_mask = static_cast<const unsigned char*>(key_mask);
-  p.mask_stride = mask_stride;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  const long total = static_cast<long>(batch) * heads * n_q;
+  p.window = g.window < (1L << 60) ? g.window : (1L << 60);
+  p.sinks = g.sinks;
+  p.causal = g.causal != 0;
+  p.lengths = g.lengths;
+  p.lengths64 = g.lengths_kind == 3;
+  p.starts = g.starts;
+  p.starts_kind = static_cast<int>(g.starts_kind);
+  p.start = clamp_long(g.start, -(1L << 60), 1L << 60);
+  p.key_mask = static_cast<const unsigned char*>(g.key_mask);
+  p.mask_stride = g.mask_stride;
+  p.scale_log2 = static_cast<float>(g.scale * 1.4426950408889634);
+  return IRIS_OK;
+}
+}  // namespace
+
+extern "C" int iris_window_attn_workspace(const iris_window_attn_args* args, long* bytes) {
+  IRIS_REQUIRE(args && bytes, "window_attn: null pointer");
+  *bytes = 0;
+  return IRIS_OK;
+}
+
+extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t stream) {
+  WindowArgs p{};
+  const int rc = window_args(args, p);
+  if (rc || p.batch == 0) return rc;
+  const long total = static_cast<long>(p.batch) * p.heads * p.n_q;
   IRIS_REQUIRE(total < (1L << 31), "window_attn: grid too large");
   window_rows_kernel<<<dim3(static_cast<unsigned>((total + 3) / 4)), 256, 0, stream>>>(p, total);
   return check_launch("window_attn");

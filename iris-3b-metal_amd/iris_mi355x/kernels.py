@@ -63,18 +63,18 @@ class _Check:
 
 
 _INT_KINDS = {torch.int32: 1, torch.int64: 3}
+_DTYPE_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
 
-def _on_current_device(op: str, first: torch.Tensor, *rest: torch.Tensor | None) -> None:
-    """All tensors on the GPU that the call's stream belongs to (the current one)."""
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError(f"{op}: the HIP kernels need GPU tensors (there is no CPU path)")
-    for t in rest:
-        if t is not None and t.device != device:
-            raise ValueError(f"{op}: tensors on {device} and on {t.device}: all must be on one GPU")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"{op}: tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+def _on_current_device(op: str, *tensors: torch.Tensor | None) -> int:
+    """Checks that all tensors are on the current GPU and returns its current stream."""
+    device = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            if not t.is_cuda:
+                raise ValueError(f"{op}: the HIP kernels need GPU tensors (there is no CPU path)")
+            raise ValueError(f"{op}: a tensor is on {t.device}, the current device is cuda:{device}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _mod_rows(vector: torch.Tensor, batch: int, width: int) -> tuple[torch.Tensor, int]:
@@ -143,66 +143,41 @@ def qk_norm_rope(
     return out
 
 
-def _rotary(op, turned, plain, outs, positions, freqs, rows, layout, factor, transpose) -> None:
-    """``iris_rotary`` of the ``turned`` tensors and the ``plain`` one (or None) into ``outs``, in that order;
-    with ``rows``, all outputs but the first go to them."""
-    xs = [*turned, plain] if plain is not None else turned
+_NO_TENSOR = (0,) * 18
+
+
+def _rotary(op, xs, outs, turned, to_rows, positions, freqs, rows, layout, factor, transpose) -> None:
+    """``iris_rotary`` of ``xs`` into ``outs``: the first ``turned`` rotate, from ``to_rows`` on tokens go to
+    ``rows``. (Shapes, strides and overlaps are checked by the library.)"""
     first = xs[0]
+    dtype = _DTYPE_CODES.get(first.dtype)
+    if dtype is None:
+        L.dtype_code(first.dtype)
+    tensors = []
+    for x, out in zip(xs, outs):
+        if x.dtype != first.dtype or out.dtype != first.dtype:
+            raise ValueError(f"{op}: heads and outputs must be of one dtype (got {x.dtype}, {out.dtype})")
+        if x.dim() != 4 or out.dim() != 4:
+            raise ValueError(f"{op}: heads must be [B, N, H, D], outputs [B, H, N, D]")
+        tensors += (x.data_ptr(), *x.shape, *x.stride(), out.data_ptr(), *out.shape, *out.stride())
     if layout not in L.ROTARY_LAYOUTS:
         raise ValueError(f"{op}: layout must be 'half' or 'interleaved', got {layout!r}")
-    if first.dim() != 4:
-        raise ValueError(f"{op}: heads must be [B, N, H, D]")
-    batch, tokens, _, dim = first.shape
-    pairs = freqs.numel()
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 0 < 2 * pairs <= dim or dim % 2:
-        raise ValueError(f"{op}: freqs must be contiguous FP64, one per rotated pair of the (even) head width {dim}")
-    x_strides, out_strides, heads, flags, out_rows = [], [], [], [], []
-    for i, (x, out) in enumerate(zip(xs, outs)):
-        if (x.dim() != 4 or x.shape[:2] != (batch, tokens) or x.shape[3] != dim or x.dtype != first.dtype
-                or (x.stride(3) != 1 and dim > 1)):
-            raise ValueError(f"{op}: heads must be [{batch}, {tokens}, H, {dim}] of one dtype with unit stride in a head")
-        to_rows = rows is not None and i > 0
-        h = x.shape[2]
-        if (out.dim() != 4 or out.shape[:2] != (batch, h) or out.shape[3] != dim or out.dtype != x.dtype
-                or out.stride(3) != 1 or (not to_rows and out.shape[2] != tokens)):
-            raise ValueError(f"{op}: output {i} must be {x.dtype} [{batch}, {h}, "
-                             f"{'rows' if to_rows else tokens}, {dim}] with unit stride in a head")
-        xs_, os_ = x.stride(), out.stride()
-        if _span_overlaps(x, out) and (to_rows or x.data_ptr() != out.data_ptr()
-                                       or (xs_[0], xs_[2], xs_[1]) != os_[:3]):
-            raise ValueError(f"{op}: output {i} must be its input itself (as [B, H, N, D]) or lie apart from it")
-        if out.shape[2] > 1 and os_[2] == 0 or h > 1 and os_[1] == 0 or batch > 1 and os_[0] == 0:
-            raise ValueError(f"{op}: output {i} is an expanded tensor")
-        x_strides += xs_[:3]
-        out_strides += os_[:3]
-        heads.append(h)
-        flags.append((L.ROTARY_TURN if i < len(turned) else 0) | (L.ROTARY_TO_ROWS if to_rows else 0))
-        out_rows.append(out.shape[2])
-    strides = []
-    for name, index in (("positions", positions), ("rows", rows)):
-        if index is None:
-            strides.append((0, 0))
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
+        raise ValueError(f"{op}: freqs must be contiguous FP64, one per rotated pair")
+    index = []
+    for name, t in (("positions", positions), ("rows", rows)):
+        if t is None:
+            index += (0, 0, 0)
             continue
-        kind = _INT_KINDS.get(index.dtype, 0)
-        if (kind == 0 or index.shape not in ((tokens,), (batch, tokens)) or (tokens > 1 and index.stride(-1) != 1)):
-            raise ValueError(f"{op}: {name} must be int32 or int64 [{batch}, {tokens}] or [{tokens}] with unit stride")
-        strides.append((kind, index.stride(0) if index.dim() == 2 else 0))
-    dtype = L.dtype_code(first.dtype)
-    _on_current_device(op, *xs, *outs, positions, freqs, rows)
-    P = L.pointer_array
-    L.call("iris_rotary", len(xs), P([x.data_ptr() for x in xs]), L.long_array(x_strides),
-           P([o.data_ptr() for o in outs]), L.long_array(out_strides), L.int_array(heads), L.int_array(flags),
-           L.long_array(out_rows), dtype, batch, tokens, dim, positions.data_ptr(), *strides[0],
-           L.ptr(rows), *strides[1], freqs.data_ptr(), pairs, L.ROTARY_LAYOUTS[layout], float(factor), bool(transpose),
-           L.stream())
-
-
-def _span_overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors meet."""
-    if not a.numel() or not b.numel():
-        return False
-    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (a, b)]
-    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+        kind, shape, wide = _INT_KINDS.get(t.dtype, 0), t.shape, t.dim() == 2
+        if (kind == 0 or t.dim() not in (1, 2) or shape[-1] != first.shape[1] or (wide and shape[0] != first.shape[0])
+                or (shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{op}: {name} must be int32 or int64 [B, N] or [N] with unit stride")
+        index += (t.data_ptr(), kind, t.stride(0) if wide else 0)
+    n = len(xs)
+    args = L.ROTARY_ARGS.pack(n, turned, to_rows, dtype, *tensors, *(_NO_TENSOR * (3 - n)), *index, freqs.data_ptr(),
+                              freqs.numel(), L.ROTARY_LAYOUTS[layout], transpose, factor)
+    L.call("iris_rotary", args, _on_current_device(op, *xs, *outs, positions, freqs, rows))
 
 
 def rotary(
@@ -226,13 +201,16 @@ def rotary(
     in FP64, the rotation in FP32. ``transpose=True`` turns the other way: the gradient with regard to the
     inputs of the call without it. ``q_out`` / ``k_out``: ``[B, H, N, D]`` views of any strides with unit
     stride inside a head; the input itself, transposed to that shape, is rotated in place."""
-    turned = [q] if k is None else [q, k]
-    for x in turned:
-        if x.dim() != 4:
-            raise ValueError("rotary: heads must be [B, N, H, D]")
-    outs = [o if o is not None else x.new_empty(x.shape[0], x.shape[2], x.shape[1], x.shape[3])
-            for x, o in zip(turned, (q_out, k_out))]
-    _rotary("rotary", turned, None, outs, positions, freqs, None, layout, factor, transpose)
+    xs = (q,) if k is None else (q, k)
+    outs = []
+    for x, out in zip(xs, (q_out, k_out)):
+        if out is None:
+            if x.dim() != 4:
+                raise ValueError("rotary: heads must be [B, N, H, D]")
+            b, n, h, d = x.shape
+            out = x.new_empty((b, h, n, d))
+        outs.append(out)
+    _rotary("rotary", xs, outs, 2, 3, positions, freqs, None, layout, factor, transpose)
     return outs[0], (outs[1] if k is not None else None)
 
 
@@ -256,11 +234,12 @@ def rotary_store(
     (as ``window_attention`` reads them). Token ``t`` of item ``b`` goes to cache row ``rows[b, t]`` (int32
     or int64, ``[B, N]`` or ``[N]``; default ``positions``), and nowhere if that row does not exist: -1 marks
     padding. All other rows stay as they are. The rows of one item must differ from each other."""
-    if q.dim() != 4:
-        raise ValueError("rotary_store: heads must be [B, N, H, D]")
     if q_out is None:
-        q_out = q.new_empty(q.shape[0], q.shape[2], q.shape[1], q.shape[3])
-    _rotary("rotary_store", [q, k], v, [q_out, k_cache, v_cache], positions, freqs,
+        if q.dim() != 4:
+            raise ValueError("rotary_store: heads must be [B, N, H, D]")
+        b, n, h, d = q.shape
+        q_out = q.new_empty((b, h, n, d))
+    _rotary("rotary_store", (q, k, v), (q_out, k_cache, v_cache), 2, 1, positions, freqs,
             positions if rows is None else rows, layout, factor, False)
     return q_out
 
@@ -800,28 +779,24 @@ def window_attention(
     A query that sees nothing gives 0. Keys that no query sees may hold anything; a query's result does
     not depend on keys it does not see, infinities and NaN among them. ``scale`` defaults to
     ``128 ** -0.5``; ``out``: BF16 ``[B, Nq, H * 128]``, unit column stride."""
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError("window_attention: q must be [B, H, Nq, 128], k and v [B, H_kv, Nk, 128] of one shape")
-    batch, heads, n_q, hd = q.shape
-    kv_heads, n_k = k.shape[1], k.shape[2]
-    if hd != HEAD_DIM or k.shape[0] != batch or k.shape[3] != HEAD_DIM or kv_heads == 0 or heads % kv_heads:
-        raise ValueError(f"window_attention: q {tuple(q.shape)} and k / v {tuple(k.shape)} do not match: one batch, "
-                         "128-wide heads, a multiple of K/V heads")
     bf16 = torch.bfloat16
     if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
         raise ValueError("window_attention: works on BF16")
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    if qs[3] != 1 or ks[3] != 1 or vs[3] != 1:
-        raise ValueError("window_attention: heads must have unit stride")
-    if (window is not None and window < 1) or sinks < 0:
-        raise ValueError(f"window_attention: window must be at least 1 (or None) and sinks nonnegative, got {window}, {sinks}")
-    lengths_kind = starts_kind = start = mask_stride = 0
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("window_attention: q must be [B, H, Nq, 128], k and v [B, H_kv, Nk, 128]")
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise ValueError(f"window_attention: window must be at least 1 (or None), got {window}")
+    q_shape, k_shape = q.shape, k.shape
+    batch, heads, n_q, _ = q_shape
+    lengths_at = lengths_kind = starts_at = starts_kind = start = mask_at = mask_stride = 0
     if lengths is not None:
-        lengths_kind = _INT_KINDS.get(lengths.dtype, 0)
+        lengths_at, lengths_kind = lengths.data_ptr(), _INT_KINDS.get(lengths.dtype, 0)
         if lengths_kind == 0 or lengths.shape != (batch,) or not lengths.is_contiguous():
             raise ValueError(f"window_attention: lengths must be contiguous int32 or int64 [{batch}]")
     if isinstance(starts, torch.Tensor):
-        starts_kind = _INT_KINDS.get(starts.dtype, 0)
+        starts_at, starts_kind = starts.data_ptr(), _INT_KINDS.get(starts.dtype, 0)
         if starts_kind == 0 or starts.shape != (batch,) or not starts.is_contiguous():
             raise ValueError(f"window_attention: starts must be an int or contiguous int32 or int64 [{batch}]")
     elif starts is not None:
@@ -829,27 +804,25 @@ def window_attention(
         if abs(start) >= 1 << 60:
             raise ValueError("window_attention: starts must lie within 2^60")
     if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (batch, n_k) or (
-                n_k > 1 and key_mask.stride(1) != 1):
-            raise ValueError(f"window_attention: key_mask must be bool or uint8 [{batch}, {n_k}] with unit column stride")
-        mask_stride = key_mask.stride(0)
-    width = heads * HEAD_DIM
-    if out is not None:
-        if out.dtype != bf16 or out.shape != (batch, n_q, width) or out.stride(2) != 1:
-            raise ValueError(f"window_attention: out must be BF16 [{batch}, {n_q}, {width}] with unit column stride")
-        out_strides = out.stride()[:2]
-        if (n_q > 1 and out_strides[1] < width) or (batch > 1 and out_strides[0] < width):
-            raise ValueError("window_attention: out's rows overlap")
-        if any(_span_overlaps(out, t) for t in (q, k, v)):
-            raise ValueError("window_attention: out must lie apart from q, k and v")
-    _on_current_device("window_attention", q, k, v, lengths, starts, key_mask, out)
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (batch, k_shape[2]) or (
+                k_shape[2] > 1 and key_mask.stride(1) != 1):
+            raise ValueError(f"window_attention: key_mask must be bool or uint8 [{batch}, {k_shape[2]}] with unit column "
+                             "stride")
+        mask_at, mask_stride = key_mask.data_ptr(), key_mask.stride(0)
     if out is None:
-        out = torch.empty(batch, n_q, width, device=q.device, dtype=bf16)
-        out_strides = (n_q * width, width)
-    L.call("iris_window_attn", q.data_ptr(), L.long_array(qs[:3]), k.data_ptr(), L.long_array(ks[:3]), v.data_ptr(),
-           L.long_array(vs[:3]), out.data_ptr(), L.long_array(out_strides), batch, heads, kv_heads, n_q, n_k,
-           min(window or 0, 1 << 60), min(sinks, 1 << 60), bool(causal), L.ptr(lengths), lengths_kind, L.ptr(starts), starts_kind, start,
-           L.ptr(key_mask), mask_stride, HEAD_DIM ** -0.5 if scale is None else float(scale), L.stream())
+        width = heads * HEAD_DIM
+        out = q.new_empty((batch, n_q, width))
+        place = (batch, n_q, width, n_q * width, width, 1)
+    elif out.dtype != bf16 or out.dim() != 3:
+        raise ValueError(f"window_attention: out must be BF16 [{batch}, {n_q}, {heads * HEAD_DIM}]")
+    else:
+        place = (*out.shape, *out.stride())
+    args = [q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *q_shape, *q.stride(), *k_shape, *k.stride(),
+            *v.shape, *v.stride(), *place, min(window, 1 << 60), min(sinks, 1 << 60), bool(causal), lengths_at,
+            lengths_kind, starts_at, starts_kind, start, mask_at, mask_stride,
+            HEAD_DIM ** -0.5 if scale is None else scale, 0, 0]
+    stream = _on_current_device("window_attention", q, k, v, out, lengths, starts, key_mask)
+    L.call("iris_window_attn", L.WINDOW_ATTN_ARGS.pack(*args), stream)
     return out
 
 
@@ -1001,13 +974,13 @@ def pack_w4(weight: torch.Tensor, group: int = 64, symmetric: bool = True,
     return (codes[:, 0::2] | codes[:, 1::2] << 4).contiguous(), scales, None if symmetric else zero.to(torch.uint8)
 
 
-def _w4_checks(op: str, codes, scales, zeros, x, bias, extra_bias, out, group: int) -> int:
-    """Checks one product of ``gemv_w4``; returns the number of its extra biases."""
+def _w4_job(op: str, codes, scales, zeros, x, bias, extra_bias, out, group: int) -> tuple:
+    """Checks one product of ``gemv_w4``; returns its ``iris_gemv_w4_job``."""
     if x.dim() != 2 or codes.dim() != 2:
         raise ValueError(f"{op}: takes [B, K] inputs and [N, K / 2] codes")
     batch, k = x.shape
-    n = codes.shape[0]
-    if codes.dtype != torch.uint8 or codes.shape[1] * 2 != k or not codes.is_contiguous():
+    n, half = codes.shape
+    if codes.dtype != torch.uint8 or half * 2 != k or not codes.is_contiguous():
         raise ValueError(f"{op}: codes must be contiguous uint8 [N, {k} / 2], two weights a byte")
     if group <= 0 or group % 32:
         raise ValueError(f"{op}: group must be a multiple of 32 (got {group})")
@@ -1018,17 +991,34 @@ def _w4_checks(op: str, codes, scales, zeros, x, bias, extra_bias, out, group: i
         raise ValueError(f"{op}: zeros must be contiguous uint8 {groups}")
     if not x.is_contiguous():
         raise ValueError(f"{op}: x must be contiguous")
-    for name, t, shape in (("bias", bias, (n,)), ("extra_bias", extra_bias, None)):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous()
-                              or (t.shape != shape if shape else t.dim() != 2 or t.shape[1] != n or t.shape[0] == 0)):
-            raise ValueError(f"{op}: {name} must be contiguous FP32 {'[N]' if shape else '[J, N]'}")
-    n_extra = 0 if extra_bias is None else extra_bias.shape[0]
-    if out.shape != ((n_extra, batch, n) if n_extra else (batch, n)) or not out.is_contiguous():
-        raise ValueError(f"{op}: out must be contiguous {(n_extra, batch, n) if n_extra else (batch, n)}")
-    if _span_overlaps(out, x):
-        raise ValueError(f"{op}: out must lie apart from x")
-    _on_current_device(op, codes, scales, zeros, x, bias, extra_bias, out)
-    return n_extra
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"{op}: bias must be contiguous FP32 [{n}]")
+    n_extra, expect = 0, (batch, n)
+    if extra_bias is not None:
+        if (extra_bias.dtype != torch.float32 or extra_bias.dim() != 2 or extra_bias.shape[1] != n
+                or extra_bias.shape[0] == 0 or not extra_bias.is_contiguous()):
+            raise ValueError(f"{op}: extra_bias must be contiguous FP32 [J, {n}]")
+        n_extra = extra_bias.shape[0]
+        expect = (n_extra, batch, n)
+    if out.shape != expect or not out.is_contiguous():
+        raise ValueError(f"{op}: out must be contiguous {expect}")
+    return (codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+            0 if bias is None else bias.data_ptr(), 0 if extra_bias is None else extra_bias.data_ptr(), out.data_ptr(),
+            n, n_extra)
+
+
+_NO_JOB = (0,) * 8
+
+
+def _w4_call(op: str, jobs: tuple, x, out, scales, group: int, in_silu: bool, out_silu: bool, *tensors) -> None:
+    codes = [_DTYPE_CODES.get(t.dtype) for t in (x, out, scales)]
+    if None in codes:
+        raise ValueError(f"{op}: x, out and scales must be FP32 or BF16")
+    batch, k = x.shape
+    args = L.GEMV_W4_ARGS.pack(len(jobs) // 8, batch, k, group, *codes, L.ACT_SILU if in_silu else L.ACT_NONE,
+                               L.ACT_SILU if out_silu else L.ACT_NONE, x.data_ptr(), *jobs,
+                               *(_NO_JOB if len(jobs) == 8 else ()))
+    L.call("iris_gemv_w4", args, _on_current_device(op, x, *tensors))
 
 
 def gemv_w4(
@@ -1051,14 +1041,8 @@ def gemv_w4(
     None for 8 everywhere. K and ``group`` are multiples of 32; the last group may be short. Sums are FP32 and,
     for FP32 inputs, of FP32 products. ``bias`` FP32 ``[N]``; ``out`` FP32 or BF16 ``[B, N]``; with
     ``extra_bias`` (``[J, N]``) ``out[j] = y + extra_bias[j]`` (``out``: ``[J, B, N]``)."""
-    n_extra = _w4_checks("gemv_w4", codes, scales, zeros, x, bias, extra_bias, out, group)
-    batch, k = x.shape
-    P = L.pointer_array
-    L.call("iris_gemv_w4", 1, P([codes.data_ptr()]), P([scales.data_ptr()]), L.dtype_code(scales.dtype),
-           P([L.ptr(zeros)]), group, x.data_ptr(), L.dtype_code(x.dtype), batch, L.int_array([codes.shape[0]]), k,
-           P([L.ptr(bias)]), P([L.ptr(extra_bias)]), L.int_array([n_extra]), P([out.data_ptr()]),
-           L.dtype_code(out.dtype), L.ACT_SILU if in_silu else L.ACT_NONE, L.ACT_SILU if out_silu else L.ACT_NONE,
-           L.stream())
+    job = _w4_job("gemv_w4", codes, scales, zeros, x, bias, extra_bias, out, group)
+    _w4_call("gemv_w4", job, x, out, scales, group, in_silu, out_silu, codes, scales, zeros, bias, extra_bias, out)
     return out
 
 
@@ -1068,17 +1052,11 @@ def gemv_w4_pair(codes, scales, x: torch.Tensor, biases, outs, group: int = 64, 
     two calls. Scales, and outputs, share a dtype."""
     lists = (codes, scales, biases, outs, zeros, extra_biases)
     _Check("gemv_w4_pair")(all(len(items) == 2 for items in lists), "takes two products")
-    n_extra = [_w4_checks("gemv_w4_pair", c, s, z, x, b, e, o, group)
-               for c, s, b, o, z, e in zip(*lists)]
+    jobs = [_w4_job("gemv_w4_pair", c, s, z, x, b, e, o, group) for c, s, b, o, z, e in zip(*lists)]
     _Check("gemv_w4_pair")(scales[0].dtype == scales[1].dtype and outs[0].dtype == outs[1].dtype,
                            "scales or outputs differ in dtype")
-    P = L.pointer_array
-    L.call("iris_gemv_w4", 2, P([c.data_ptr() for c in codes]), P([s.data_ptr() for s in scales]),
-           L.dtype_code(scales[0].dtype), P([L.ptr(z) for z in zeros]), group, x.data_ptr(), L.dtype_code(x.dtype),
-           x.shape[0], L.int_array([c.shape[0] for c in codes]), x.shape[1], P([L.ptr(b) for b in biases]),
-           P([L.ptr(e) for e in extra_biases]), L.int_array(n_extra), P([o.data_ptr() for o in outs]),
-           L.dtype_code(outs[0].dtype), L.ACT_SILU if in_silu else L.ACT_NONE, L.ACT_SILU if out_silu else L.ACT_NONE,
-           L.stream())
+    _w4_call("gemv_w4_pair", jobs[0] + jobs[1], x, outs[0], scales[0], group, in_silu, out_silu,
+             *(t for items in lists for t in items))
 
 
 def timestep_gemv(t: torch.Tensor, freqs: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, out: torch.Tensor,

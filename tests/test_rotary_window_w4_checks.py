@@ -10,6 +10,19 @@ from iris_mi355x import tables
 BF16 = torch.bfloat16
 
 
+@pytest.fixture
+def unplaced(monkeypatch):
+    """Without the check for GPU tensors, so that the library's own refusals are reached (each comes before
+    anything is launched)."""
+    monkeypatch.setattr(K, "_on_current_device", lambda op, *tensors: 0)
+
+
+def test_cpu_tensors_are_refused():
+    for call in (attention, rotary, w4):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+
+
 def attention(**change):
     args = dict(q=torch.zeros(2, 4, 3, 128, dtype=BF16), k=torch.zeros(2, 2, 9, 128, dtype=BF16),
                 v=torch.zeros(2, 2, 9, 128, dtype=BF16))
@@ -18,7 +31,6 @@ def attention(**change):
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(), "GPU"),
     (dict(q=torch.zeros(2, 4, 3, 64, dtype=BF16)), "do not match"),
     (dict(q=torch.zeros(2, 3, 3, 128, dtype=BF16)), "do not match"),
     (dict(q=torch.zeros(1, 4, 3, 128, dtype=BF16)), "do not match"),
@@ -40,7 +52,7 @@ def attention(**change):
     (dict(out=torch.zeros(2, 3, 512)), "out"),
     (dict(out=torch.zeros(2, 4, 512, dtype=BF16)), "out"),
 ])
-def test_window_attention_refuses(change, match):
+def test_window_attention_refuses(unplaced, change, match):
     with pytest.raises(ValueError, match=match):
         attention(**change)
 
@@ -53,10 +65,9 @@ def rotary(**change):
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(), "GPU"),
     (dict(layout="pairs"), "layout"),
-    (dict(freqs=torch.zeros(33, dtype=torch.float64)), "freqs"),
-    (dict(freqs=torch.zeros(0, dtype=torch.float64)), "freqs"),
+    (dict(freqs=torch.zeros(33, dtype=torch.float64)), "33 rotated pairs"),
+    (dict(freqs=torch.zeros(0, dtype=torch.float64)), "rotated pairs"),
     (dict(freqs=torch.zeros(32)), "freqs"),
     (dict(q=torch.zeros(2, 5, 256)), "heads"),
     (dict(q=torch.zeros(2, 5, 4, 63), k=None, freqs=torch.zeros(4, dtype=torch.float64)), "even"),
@@ -67,21 +78,19 @@ def rotary(**change):
     (dict(positions=torch.zeros(5, 2, dtype=torch.int64).T), "positions"),
     (dict(positions=torch.zeros(3, 5, dtype=torch.int64)), "positions"),
     (dict(q_out=torch.zeros(2, 4, 6, 64)), "output 0"),
-    (dict(k_out=torch.zeros(2, 2, 5, 64, dtype=BF16)), "output 1"),
+    (dict(k_out=torch.zeros(2, 2, 5, 64, dtype=BF16)), "one dtype"),
     (dict(q_out=torch.zeros(1, 4, 5, 64).expand(2, -1, -1, -1)), "expanded"),
     (dict(q=torch.zeros(2, 5, 4, 64, dtype=torch.float16), k=None), "float32 or bfloat16"),
 ])
-def test_rotary_refuses(change, match):
+def test_rotary_refuses(unplaced, change, match):
     with pytest.raises(ValueError, match=match):
         rotary(**change)
 
 
-def test_rotary_refuses_an_output_that_meets_its_input():
+def test_rotary_refuses_an_output_that_meets_its_input(unplaced):
     x = torch.zeros(2, 6, 4, 64)
     with pytest.raises(ValueError, match="itself"):
         rotary(q=x[:, :5], k=None, q_out=x[:, 1:].transpose(1, 2))
-    with pytest.raises(ValueError, match="GPU"):  # in place is not refused
-        rotary(q=x[:, :5], k=None, q_out=x[:, :5].transpose(1, 2))
     q, k = torch.zeros(2, 5, 4, 64), torch.zeros(2, 5, 2, 64)
     args = (torch.zeros(5, dtype=torch.int64), torch.zeros(32, dtype=torch.float64))
     with pytest.raises(ValueError, match="itself"):  # rows move
@@ -101,7 +110,6 @@ def w4(**change):
 
 
 @pytest.mark.parametrize("change,match", [
-    (dict(), "GPU"),
     (dict(codes=torch.zeros(6, 64, dtype=torch.int8)), "codes"),
     (dict(codes=torch.zeros(6, 63, dtype=torch.uint8)), "codes"),
     (dict(codes=torch.zeros(6, 128, dtype=torch.uint8)[:, ::2]), "codes"),
@@ -118,7 +126,7 @@ def w4(**change):
     (dict(extra_bias=torch.zeros(0, 6)), "extra_bias"),
     (dict(out=torch.zeros(6, 3)), "out"),
 ])
-def test_gemv_w4_refuses(change, match):
+def test_gemv_w4_refuses(unplaced, change, match):
     with pytest.raises(ValueError, match=match):
         w4(**change)
 
@@ -157,40 +165,60 @@ def test_rotary_frequencies():
             tables.rotary_frequencies(**{"dim": 8, "theta": 100.0, "device": "cpu", **bad})
 
 
+def test_out_apart_from_inputs(unplaced):
+    store = torch.zeros(2, 3, 4, 128, dtype=BF16)
+    with pytest.raises(ValueError, match="apart"):
+        attention(q=store.transpose(1, 2), out=store.flatten(2))
+    x = torch.zeros(128 * 64)
+    with pytest.raises(ValueError, match="apart"):
+        w4(x=x[:384].view(3, 128), out=x[380:398].view(3, 6))
+
+
 def test_c_entry_points_refuse():
     """What the library itself turns away, before any launch (pointers are never followed)."""
     at = 1 << 20
-    longs, ints, pointers = _lib.long_array, _lib.int_array, _lib.pointer_array
-    s3 = longs([1024, 128, 128])
+    names = {
+        "iris_window_attn": (_lib.WINDOW_ATTN_ARGS, dict(
+            q=at, k=at, v=at, out=1 << 30, q_shape=(2, 4, 3, 128), q_strides=(1536, 384, 128, 1), k_shape=(2, 2, 9, 128),
+            k_strides=(2304, 1152, 128, 1), v_shape=(2, 2, 9, 128), v_strides=(2304, 1152, 128, 1), out_shape=(2, 3, 512),
+            out_strides=(1536, 512, 1), window=0, sinks=0, causal=1, lengths=0, lengths_kind=0, starts=0, starts_kind=0,
+            start=0, key_mask=0, mask_stride=0, scale=0.1, workspace=0, workspace_bytes=0)),
+        "iris_rotary": (_lib.ROTARY_ARGS, dict(
+            tensors=1, turned=1, to_rows=3, dtype=0, x=at, x_shape=(2, 5, 2, 64), x_strides=(640, 128, 64, 1), out=1 << 30,
+            out_shape=(2, 2, 5, 64), out_strides=(640, 320, 64, 1), rest=(0,) * 36, positions=at, positions_kind=1,
+            positions_stride=5, rows=0, rows_kind=0, rows_stride=0, freqs=at, pairs=32, layout=0, transpose=0, factor=1.0)),
+        "iris_gemv_w4": (_lib.GEMV_W4_ARGS, dict(
+            jobs=1, batch=1, k=128, group=64, x_dtype=0, out_dtype=0, scales_dtype=1, in_act=0, out_act=0, x=at, codes=at,
+            scales=at, zeros=0, bias=0, extra_bias=0, out=1 << 30, n=6, n_extra=0, rest=(0,) * 8)),
+    }
 
-    def attn(q=at, heads=4, kv=2, nq=3, nk=9, window=0, sinks=0, qs=s3, lengths_kind=0, lengths=None, starts=None,
-             starts_kind=0):
-        _lib.call("iris_window_attn", q, qs, at, s3, at, s3, at, longs([2048, 512]), 2, heads, kv, nq, nk, window, sinks, 1,
-                  lengths, lengths_kind, starts, starts_kind, 0, None, 0, 0.1, None)
-
-    for change, match in ((dict(heads=3), "multiple"), (dict(nk=1 << 30), "2\\^30"), (dict(window=-1), "negative"),
-                          (dict(q=at + 8), "aligned"), (dict(q=None), "null"), (dict(qs=longs([1024, 128, 4])), "strides"),
-                          (dict(lengths=at, lengths_kind=2), "lengths"), (dict(starts_kind=1), "starts")):
+    def refused(name, match, **change):
+        layout, args = names[name]
+        values = []
+        for value in {**args, **change}.values():
+            values += value if isinstance(value, tuple) else (value,)
         with pytest.raises(ValueError, match=match):
-            attn(**change)
+            _lib.call(name, layout.pack(*values), None)
 
-    def turn(tensors=1, dim=64, pairs=32, layout=0, flags=1, rows=None, kind=1, out_rows=5, x=at):
-        _lib.call("iris_rotary", tensors, pointers([x]), longs([640, 128, 64]), pointers([at]), longs([640, 320, 64]),
-                  ints([2]), ints([flags]), longs([out_rows]), _lib.F32, 2, 5, dim, at, kind, 5, rows, 1, 0, at, pairs,
-                  layout, 1.0, 0, None)
-
-    for change, match in ((dict(tensors=0), "one to three"), (dict(tensors=4), "one to three"), (dict(dim=63), "even"),
-                          (dict(pairs=33), "head width"), (dict(layout=2), "layout"), (dict(flags=3), "rows"),
-                          (dict(kind=2), "positions"), (dict(out_rows=4), "fewer rows"), (dict(x=None), "null")):
-        with pytest.raises(ValueError, match=match):
-            turn(**change)
-
-    def gemv(jobs=1, group=64, k=128, codes=at, extra=0, x=at, act=0):
-        _lib.call("iris_gemv_w4", jobs, pointers([codes]), pointers([at]), _lib.BF16, pointers([None]), group, x, _lib.F32,
-                  1, ints([6]), k, pointers([None]), pointers([None]), ints([extra]), pointers([at]), _lib.F32, act, 0, None)
-
+    for change, match in ((dict(q_shape=(2, 3, 3, 128)), "multiple"), (dict(k_shape=(2, 2, 1 << 30, 128)), "one shape"),
+                          (dict(k_shape=(2, 2, 1 << 30, 128), v_shape=(2, 2, 1 << 30, 128)), "2\\^30"),
+                          (dict(window=-1), "negative"), (dict(q=at + 8), "aligned"), (dict(q=0), "null"),
+                          (dict(q_strides=(1024, 128, 4, 1)), "strides"), (dict(k_strides=(2304, 1152, 128, 2)), "unit"),
+                          (dict(lengths=at, lengths_kind=2), "lengths"), (dict(starts_kind=1), "starts"),
+                          (dict(out_strides=(1536, 256, 1)), "overlap"), (dict(out=at), "apart"),
+                          (dict(out_shape=(2, 3, 511)), "out must be")):
+        refused("iris_window_attn", match, **change)
+    for change, match in ((dict(tensors=0), "one to three"), (dict(tensors=4), "one to three"), (dict(dtype=2), "dtype"),
+                          (dict(x_shape=(2, 5, 2, 63)), "even"), (dict(pairs=33), "head width"), (dict(layout=2), "layout"),
+                          (dict(to_rows=0), "rows"), (dict(positions_kind=2), "positions"),
+                          (dict(out_shape=(2, 2, 4, 64)), "output 0"), (dict(x=0), "null"), (dict(freqs=0), "null"),
+                          (dict(out=at + 4), "itself"), (dict(out_strides=(0, 320, 64, 1)), "expanded")):
+        refused("iris_rotary", match, **change)
     for change, match in ((dict(jobs=3), "one or two"), (dict(group=48), "multiple of 32"), (dict(k=48), "k % 32"),
-                          (dict(codes=at + 4), "aligned"), (dict(codes=None), "null"), (dict(extra=2), "extra"),
-                          (dict(x=None), "input"), (dict(act=2), "activation")):
-        with pytest.raises(ValueError, match=match):
-            gemv(**change)
+                          (dict(codes=at + 4), "aligned"), (dict(codes=0), "null"), (dict(n_extra=2), "extra"), (dict(n=0), "rows"),
+                          (dict(x=0), "input"), (dict(x=at + 4), "aligned"), (dict(in_act=2), "activation"),
+                          (dict(x_dtype=2), "dtype"), (dict(out=at + 8), "apart")):
+        refused("iris_gemv_w4", match, **change)
+    for name in names:
+        with pytest.raises(ValueError, match="null"):
+            _lib.call(name, None, None)
