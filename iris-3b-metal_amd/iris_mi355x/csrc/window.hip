@@ -6,6 +6,19 @@
 // so a query's keys are [0, sink_end) and [low, high) less the masked ones (Span). The result is
 //   o = sum_j exp(scale q.k_j - m) v_j / sum_j exp(scale q.k_j - m) over its visible keys (m their largest
 //   score), and 0 where nothing is visible.
+//
+// One pass over the keys with a running maximum and sum, tile by tile (Attend): S^T = K Q^T and O^T = V^T P^T
+// on v_mfma_f32_16x16x32_bf16, a lane owning one query and four keys of every 16, so that P^T stays in the
+// registers it was computed in. K and V arrive as rows (views of a projection or a cache) and go straight
+// into LDS; V^T fragments are read from the V rows by the transposing LDS read (four rows by 16 columns per
+// 16 lanes). Only tiles that hold a visible key of some query of the workgroup are visited.
+//
+// window_attn_kernel (prompts): bound by the MFMAs and the softmax beside them. A workgroup's waves share a
+// ring of K/V tiles; a wave is one query head's 32 rows, the heads of a K/V head side by side.
+// window_few_kernel (few queries): bound by the keys' and values' way from memory. The rows of a tile are the
+// (query, head) pairs of one K/V head; every wave streams key tiles of its own through its own LDS, without
+// barriers, and the waves' and workgroups' parts are joined at the end (window_join_kernel for the latter).
+// window_rows_kernel: row strides too large for the 32-bit offsets of the others.
 #include "iris_common.hpp"
 
 namespace iris {
@@ -26,7 +39,14 @@ struct WindowArgs {
   const unsigned char* key_mask;
   long mask_stride;
   float scale_log2;
+  int hpw, rows_per_wg, n_qblocks, n_hgroups;  // window_attn_kernel
+  int total_wg;
+  int splits, row_tiles;  // window_few_kernel
+  float *part_o, *part_ml;  // [row][split][128] and [row][split][2] of the split form
 };
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 __host__ __device__ __forceinline__ long clamp_long(long x, long lo, long hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
@@ -55,6 +75,485 @@ __device__ __forceinline__ Span span_of(const WindowArgs& p, long pos, int lengt
   s.sink_end = p.window ? static_cast<int>(clamp_long(p.causal && pos + 1 < p.sinks ? pos + 1 : p.sinks, 0, length)) : 0;
   if (s.low < s.sink_end) s.low = s.sink_end;
   return s;
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+// Lane i of 16 gets column i of the 4 x 16 block whose row j the lanes 4 j .. 4 j + 3 address, 8 bytes each.
+__device__ __forceinline__ bf16x4 read_tr(const char* p) {
+  return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+// The bytes of `rows` rows of 128 values `stride` elements apart as a buffer: reads past them give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const bf16* p, long rows, long stride) {
+  const long bytes = rows <= 0 ? 0 : (rows - 1) * stride * 2 + 2 * kHd;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, static_cast<int>(bytes < 0x7fffffffL ? bytes : 0x7fffffffL),
+                                           kBufferFlags);
+}
+
+// 16-byte chunk c of row r of a tile lies at chunk c ^ swz of that row in LDS: the 16 rows of a K fragment read
+// (one chunk each) and the 8 rows that 32 lanes of a transposing V read touch (two chunks each) then start in
+// distinct banks.
+__device__ __forceinline__ int k_swz(int row) { return row & 15; }
+__device__ __forceinline__ int v_swz(int row) { return 2 * (row & 7); }
+
+__device__ __forceinline__ bool any_odd(u16x2 top) { return top[0] >= 0x7f80 || top[1] >= 0x7f80; }
+
+// The running attention of 16 RB queries of one head per wave over tiles of KVT keys in LDS (K rows, then V rows,
+// 256 bytes each). Lane l (l16 = l % 16, h = l / 16) owns queries 16 qb + l16 and, of each 16 keys of a tile, keys
+// 4 h .. 4 h + 3: s[kb][qb][e] is key 16 kb + 4 h + e. The keys of a P V step (32 of them) are taken in the order
+// 16 (j / 4) + 4 h + j % 4 for k-index 8 h + j, in P^T and V^T alike. o[db][qb][e] is dim 16 db + 4 h + e.
+template <int RB, int KVT>
+struct Attend {
+  static constexpr int NKB = KVT / 16, H32 = KVT / 32;
+  bf16x8 qf[RB][4];  // query 16 qb + l16, dims 32 st + 8 h .. + 8
+  f32x4 o[8][RB];
+  float m[RB], l[RB];  // log2 domain; l: this lane's keys only
+  Span span[RB];
+  int k_rd[4], v_rd[8];
+  int l16, h;
+  float sl2;  // > 0
+
+  // The scale's sign goes into the queries (and a scale of 0 turns them into zeros).
+  __device__ __forceinline__ void load_query(int qb, const bf16* row, float scale_log2) {
+    sl2 = scale_log2 == 0.0f ? 1.0f : __builtin_fabsf(scale_log2);
+    const unsigned flip = scale_log2 < 0.0f ? 0x80008000u : 0u, keep = scale_log2 == 0.0f ? 0u : ~0u;
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      uint4 v = *reinterpret_cast<const uint4*>(row + 32 * st + 8 * h);
+      v = uint4{(v.x ^ flip) & keep, (v.y ^ flip) & keep, (v.z ^ flip) & keep, (v.w ^ flip) & keep};
+      qf[qb][st] = __builtin_bit_cast(bf16x8, v);
+    }
+  }
+  __device__ __forceinline__ void start(int lane) {
+    l16 = lane & 15, h = lane >> 4;
+#pragma unroll
+    for (int qb = 0; qb < RB; ++qb) m[qb] = -INFINITY, l[qb] = 0.0f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+#pragma unroll
+      for (int qb = 0; qb < RB; ++qb) o[db][qb] = f32x4{};
+#pragma unroll
+    for (int st = 0; st < 4; ++st) k_rd[st] = l16 * 256 + 16 * ((4 * st + h) ^ k_swz(l16));
+    const int row = 4 * h + (l16 >> 2);
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+      v_rd[db] = row * 256 + 16 * ((2 * db + ((l16 & 3) >> 1)) ^ v_swz(row)) + 8 * (l16 & 1);
+  }
+  __device__ __forceinline__ bool visible(int qb, int j, unsigned long long keys, int in_tile) const {
+    return (j < span[qb].sink_end || (j >= span[qb].low && j < span[qb].high)) && (keys >> in_tile & 1);
+  }
+  __device__ __forceinline__ bf16x8 v_frag(const char* vl, int hf, int db) const {
+    const bf16x4 a = read_tr(vl + hf * 32 * 256 + v_rd[db]), b = read_tr(vl + (hf * 32 + 16) * 256 + v_rd[db]);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+
+  // PARTIAL: some query may not see some key; `keys` has a bit for every key of the tile that the key mask shows.
+  template <bool PARTIAL>
+  __device__ __forceinline__ void tile(const char* kl, const char* vl, int kv0, unsigned long long keys) {
+    f32x4 s[NKB][RB];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int qb = 0; qb < RB; ++qb) s[kb][qb] = f32x4{};
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) {
+        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kl + kb * 16 * 256 + k_rd[st]);
+#pragma unroll
+        for (int qb = 0; qb < RB; ++qb)
+          s[kb][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qb][st], s[kb][qb], 0, 0, 0);
+      }
+    if constexpr (PARTIAL) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 16 * kb + 4 * h + e;
+#pragma unroll
+          for (int qb = 0; qb < RB; ++qb)
+            if (!visible(qb, kv0 + i, keys, i)) s[kb][qb][e] = -INFINITY;
+        }
+    }
+
+    // Online softmax against a running maximum that is raised lazily: while a lane's exponentials of the tile add
+    // up to at most 2^8 the maximum and the output stay as they are; otherwise the queries that need it take their
+    // exact maxima, rescale, and recompute. A query with no key so far keeps -inf, and its hidden keys are taken
+    // against 0, which makes them exact zeros instead of NaN. The sums add the FP32 exponentials; P is rounded to
+    // BF16 (the MFMA's operand) after that.
+    bf16x8 pf[H32][RB];
+    auto probs = [&](int qb, float ref) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qb][e], sl2, -ref));
+          pf[kb / 2][qb][4 * (kb % 2) + e] = from_f32<bf16>(x);
+          sum += x;
+        }
+      return sum;
+    };
+#pragma unroll
+    for (int qb = 0; qb < RB; ++qb) {
+      float sum = probs(qb, m[qb]);
+      const int need = !(sum <= 256.0f);  // also for NaN (the first tile, a hidden key of a query without keys)
+      if (__any(need)) {
+        int raise = need | __shfl_xor(need, 16);
+        raise |= __shfl_xor(raise, 32);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[kb][qb][e]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float m_new = raise ? fmaxf(m[qb], mx * sl2) : m[qb];
+        const float ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m[qb] - ref);  // exactly 1 unless raised
+        l[qb] *= alpha;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) o[db][qb] *= alpha;
+        m[qb] = m_new;
+        sum = probs(qb, ref);
+      }
+      l[qb] += sum;
+    }
+
+    if constexpr (PARTIAL) {
+      // A value that is not finite reaches every query of the MFMA (0 times NaN): where the tile holds one, it is
+      // left out of the products and added to the queries that see it.
+      u16x2 top{0, 0};
+#pragma unroll
+      for (int i = 0; i < 8 * H32; ++i) {
+        const uint4 v = __builtin_bit_cast(uint4, v_frag(vl, i / 8, i % 8));
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.x & 0x7fff7fffu));
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.y & 0x7fff7fffu));
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.z & 0x7fff7fffu));
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.w & 0x7fff7fffu));
+      }
+      if (__any(any_odd(top))) {
+#pragma unroll
+        for (int i = 0; i < 8 * H32; ++i) {
+          bf16x8 v = v_frag(vl, i / 8, i % 8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (!__builtin_isfinite(to_f32(v[e]))) v[e] = from_f32<bf16>(0.0f);
+#pragma unroll
+          for (int qb = 0; qb < RB; ++qb)
+            o[i % 8][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[i / 8][qb], o[i % 8][qb], 0, 0, 0);
+        }
+#pragma unroll 1
+        for (int key = 0; key < KVT; ++key)
+#pragma unroll
+          for (int db = 0; db < 8; ++db) {
+            const int d = 16 * db + 4 * h;
+            const f32x4 v = load4(reinterpret_cast<const bf16*>(vl + key * 256 + 16 * ((d >> 3) ^ v_swz(key)) + 2 * (d & 7)));
+#pragma unroll
+            for (int qb = 0; qb < RB; ++qb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!__builtin_isfinite(v[e]) && visible(qb, kv0 + key, keys, key)) o[db][qb][e] += v[e];
+          }
+        return;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8 * H32; ++i) {
+      const bf16x8 vf = v_frag(vl, i / 8, i % 8);
+#pragma unroll
+      for (int qb = 0; qb < RB; ++qb)
+        o[i % 8][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[i / 8][qb], o[i % 8][qb], 0, 0, 0);
+    }
+  }
+};
+
+// The tiles that hold a visible key of queries at positions first .. last: those of [0, sinks), then those of
+// [low, high) that are not among them.
+template <int KVT>
+struct Tiles {
+  int sink, band, count;
+  __device__ __forceinline__ Tiles(const WindowArgs& p, long first, long last, int length) {
+    const Span a = span_of(p, first, length), z = span_of(p, last, length);
+    sink = (z.sink_end + KVT - 1) / KVT;
+    band = max(a.low / KVT, sink);
+    count = sink + max((z.high + KVT - 1) / KVT - band, 0);
+    if (a.low >= z.high) count = sink;
+  }
+  __device__ __forceinline__ int key(int t) const { return (t < sink ? t : t - sink + band) * KVT; }
+};
+// Whether queries at positions with the spans a (the first) .. z (the last) see all, or none, of a tile.
+template <int KVT>
+__device__ __forceinline__ bool sees_all(const Span& a, const Span& z, int kv0) {
+  return kv0 + KVT <= a.sink_end || (kv0 >= z.low && kv0 + KVT <= a.high);
+}
+template <int KVT>
+__device__ __forceinline__ bool sees_none(const Span& a, const Span& z, int kv0) {
+  return kv0 >= z.sink_end && (kv0 >= z.high || kv0 + KVT <= a.low);
+}
+
+// A bit for every key of the tile at kv0 that the mask shows, from one byte per lane.
+__device__ __forceinline__ int mask_byte(const unsigned char* mask, int kv0, int lane, int length) {
+  return kv0 + lane < length ? mask[kv0 + lane] : 0;
+}
+
+template <int NW, int STAGES, int KVT, bool MASK>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 12 ? 3 : 2))) void
+window_attn_kernel(WindowArgs p) {
+  constexpr int STAGE = 2 * KVT * 256;  // bytes: K rows, then V rows
+  constexpr int LOADS = KVT / 16;       // 1 KB loads (4 rows) per fetching wave and operand; the first four waves fetch
+  constexpr int LPW = 2 * LOADS;
+  static_assert((KVT == 32 || KVT == 64) && STAGES >= 2 && (STAGES - 2) * LPW < 64, "pipeline");
+  __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+
+  // logical workgroup: (item, K/V head, head group) major, query block minor and, where later queries see more
+  // keys, the last block first; one K/V head's blocks stay on one XCD
+  int wg = xcd_remap(blockIdx.x, p.total_wg);
+  int qblk = wg % p.n_qblocks;
+  if (p.causal) qblk = p.n_qblocks - 1 - qblk;
+  wg /= p.n_qblocks;
+  const int hg = wg % p.n_hgroups;
+  wg /= p.n_hgroups;
+  const int kvh = wg % p.kv_heads;
+  const int b = wg / p.kv_heads;
+
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hd = kvh * (p.heads / p.kv_heads) + hg * p.hpw + w % p.hpw;
+  const int length = __builtin_amdgcn_readfirstlane(item_length(p, b));
+  const long pos0 = item_start(p, b, length);
+  const int wg0 = qblk * p.rows_per_wg;
+  const int q0 = wg0 + (w / p.hpw) * 32;
+
+  Attend<2, KVT> at;
+  at.start(lane);
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int row = min(q0 + 16 * qb + at.l16, p.n_q - 1);
+    at.load_query(qb, p.q + b * p.qs_b + hd * p.qs_h + row * p.qs_n, p.scale_log2);
+    at.span[qb] = span_of(p, pos0 + row, length);
+  }
+  const Tiles<KVT> tiles(p, pos0 + wg0, pos0 + min(wg0 + p.rows_per_wg, p.n_q) - 1, length);
+  const Span first = span_of(p, pos0 + min(q0, p.n_q - 1), length), last = span_of(p, pos0 + min(q0 + 31, p.n_q - 1), length);
+  const bool idle = q0 >= p.n_q;
+
+  const bf16* kh = p.k + b * p.ks_b + kvh * p.ks_h;
+  const bf16* vh = p.v + b * p.vs_b + kvh * p.vs_h;
+  const unsigned char* mask = MASK ? p.key_mask + b * p.mask_stride : nullptr;
+  int k_off[LOADS], v_off[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int r = (w * LOADS + j) * 4 + (lane >> 4);
+    k_off[j] = r * static_cast<int>(p.ks_n) * 2 + 16 * ((lane & 15) ^ k_swz(r));
+    v_off[j] = r * static_cast<int>(p.vs_n) * 2 + 16 * ((lane & 15) ^ v_swz(r));
+  }
+  auto issue = [&](int t, int stage) {
+    if (NW != 4 && w >= 4) return;
+    const int kv0 = tiles.key(t);
+    const __amdgpu_buffer_rsrc_t rk = rows_buffer(kh + kv0 * p.ks_n, length - kv0, p.ks_n);
+    const __amdgpu_buffer_rsrc_t rv = rows_buffer(vh + kv0 * p.vs_n, length - kv0, p.vs_n);
+    bf16* kl = reinterpret_cast<bf16*>(lds + stage * STAGE);
+    bf16* vl = kl + KVT * kHd;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      buffer_load_lds16(rk, kl + (w * LOADS + j) * 512, k_off[j], 0);
+      buffer_load_lds16(rv, vl + (w * LOADS + j) * 512, v_off[j], 0);
+    }
+  };
+
+  const int n_tiles = tiles.count;
+  int byte = MASK && n_tiles > 0 ? mask_byte(mask, tiles.key(0), lane, length) : 0;
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < n_tiles) issue(s, s);
+  for (int t = 0, stage = 0; t < n_tiles; ++t, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+    unsigned long long keys = ~0ull;
+    if (MASK) {
+      keys = __ballot(byte != 0);
+      if (t + 1 < n_tiles) byte = mask_byte(mask, tiles.key(t + 1), lane, length);
+    }
+    if (t + STAGES - 2 < n_tiles)
+      wait_vmcnt<(STAGES - 2) * LPW>();
+    else
+      wait_vmcnt<0>();
+    __builtin_amdgcn_s_barrier();  // tile t is there; the stage of tile t - 1 is no longer read
+    asm volatile("" ::: "memory");
+    if (t + STAGES - 1 < n_tiles) issue(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+    const int kv0 = tiles.key(t);
+    if (idle || sees_none<KVT>(first, last, kv0)) continue;
+    constexpr unsigned long long kAll = KVT == 64 ? ~0ull : (1ull << (KVT & 63)) - 1;
+    if (MASK && !(keys & kAll)) continue;
+    const char* kl = lds + stage * STAGE;
+    if (sees_all<KVT>(first, last, kv0) && (!MASK || (keys & kAll) == kAll))
+      at.template tile<false>(kl, kl + KVT * 256, kv0, keys);
+    else
+      at.template tile<true>(kl, kl + KVT * 256, kv0, keys);
+  }
+
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    float l = at.l[qb] + __shfl_xor(at.l[qb], 16);
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int row = q0 + 16 * qb + at.l16;
+    if (row >= p.n_q) continue;
+    bf16* out = p.out + b * p.os_b + row * p.os_n + hd * kHd + 4 * at.h;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) store4(out + 16 * db, at.o[db][qb] * inv);
+  }
+}
+
+// Few queries: the 16 rows of a wave's tile are (query, head of the group) pairs r = t group + g of one K/V head.
+constexpr int kFewWaves = 4, kFewKeys = 32, kFewStages = 2;
+constexpr int kMaxSplits = 64;
+
+template <bool MASK>
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(1))) void window_few_kernel(WindowArgs p) {
+  constexpr int KVT = kFewKeys, STAGE = 2 * KVT * 256, LOADS = KVT / 4, LPW = 2 * LOADS;
+  __shared__ __attribute__((aligned(1024))) char lds[kFewWaves * kFewStages * STAGE];
+  __shared__ float ml[kFewWaves][16][2];
+
+  int wg = xcd_remap(blockIdx.x, p.total_wg);
+  const int rt = wg % p.row_tiles;
+  wg /= p.row_tiles;
+  const int split = wg % p.splits;
+  wg /= p.splits;
+  const int kvh = wg % p.kv_heads;
+  const int b = wg / p.kv_heads;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = p.heads / p.kv_heads, rows = group * p.n_q;
+  const int length = __builtin_amdgcn_readfirstlane(item_length(p, b));
+  const long pos0 = item_start(p, b, length);
+
+  Attend<1, KVT> at;
+  at.start(lane);
+  const int row = min(rt * 16 + at.l16, rows - 1), t_row = row / group, hd = kvh * group + row - t_row * group;
+  at.load_query(0, p.q + b * p.qs_b + hd * p.qs_h + t_row * p.qs_n, p.scale_log2);
+  at.span[0] = span_of(p, pos0 + t_row, length);
+  const long pos_a = pos0 + rt * 16 / group, pos_z = pos0 + min(rt * 16 + 15, rows - 1) / group;
+  const Span first = span_of(p, pos_a, length), last = span_of(p, pos_z, length);
+  const Tiles<KVT> tiles(p, pos_a, pos_z, length);
+  const int per = (tiles.count + p.splits - 1) / p.splits;
+  const int end = min(tiles.count, (split + 1) * per);
+
+  const bf16* kh = p.k + b * p.ks_b + kvh * p.ks_h;
+  const bf16* vh = p.v + b * p.vs_b + kvh * p.vs_h;
+  const unsigned char* mask = MASK ? p.key_mask + b * p.mask_stride : nullptr;
+  int k_off[LOADS], v_off[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int r = j * 4 + (lane >> 4);
+    k_off[j] = r * static_cast<int>(p.ks_n) * 2 + 16 * ((lane & 15) ^ k_swz(r));
+    v_off[j] = r * static_cast<int>(p.vs_n) * 2 + 16 * ((lane & 15) ^ v_swz(r));
+  }
+  char* const mine = lds + w * kFewStages * STAGE;
+  auto issue = [&](int t, int stage) {
+    const int kv0 = tiles.key(t);
+    const __amdgpu_buffer_rsrc_t rk = rows_buffer(kh + kv0 * p.ks_n, length - kv0, p.ks_n);
+    const __amdgpu_buffer_rsrc_t rv = rows_buffer(vh + kv0 * p.vs_n, length - kv0, p.vs_n);
+    bf16* kl = reinterpret_cast<bf16*>(mine + stage * STAGE);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) buffer_load_lds16(rk, kl + j * 512, k_off[j], 0);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) buffer_load_lds16(rv, kl + KVT * kHd + j * 512, v_off[j], 0);
+  };
+  int t = split * per + w;
+  int byte = MASK && t < end ? mask_byte(mask, tiles.key(t), lane, length) : 0;
+  if (t < end) issue(t, 0);
+  for (int stage = 0; t < end; t += kFewWaves, stage ^= 1) {
+    unsigned long long keys = ~0ull;
+    if (MASK) keys = __ballot(byte != 0);
+    if (t + kFewWaves < end) {
+      if (MASK) byte = mask_byte(mask, tiles.key(t + kFewWaves), lane, length);
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage's last reads are done
+      issue(t + kFewWaves, stage ^ 1);
+      wait_vmcnt<LPW>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    asm volatile("" ::: "memory");
+    const int kv0 = tiles.key(t);
+    constexpr unsigned long long kAll = (1ull << KVT) - 1;
+    if (MASK && !(keys & kAll)) continue;
+    const char* kl = mine + stage * STAGE;
+    if (sees_all<KVT>(first, last, kv0) && (!MASK || (keys & kAll) == kAll))
+      at.template tile<false>(kl, kl + KVT * 256, kv0, keys);
+    else
+      at.template tile<true>(kl, kl + KVT * 256, kv0, keys);
+  }
+
+  // join the waves: every wave's sums against the largest of their maxima, then one thread per 8 dims of a row
+  float l = at.l[0] + __shfl_xor(at.l[0], 16);
+  l += __shfl_xor(l, 32);
+  if (lane < 16) ml[w][lane][0] = at.m[0], ml[w][lane][1] = l;
+  __syncthreads();  // (the rings are no longer read)
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) top = fmaxf(top, ml[i][at.l16][0]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  const float mine_scale = __builtin_amdgcn_exp2f(at.m[0] - ref);
+  float* const sums = reinterpret_cast<float*>(lds) + w * 16 * 132;  // rows of 132: distinct banks
+#pragma unroll
+  for (int db = 0; db < 8; ++db) store4(sums + at.l16 * 132 + 16 * db + 4 * at.h, at.o[db][0] * mine_scale);
+  __syncthreads();
+  const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
+  if (rt * 16 + r >= rows) return;
+  float acc[8] = {}, lsum = 0.0f, rtop = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) rtop = fmaxf(rtop, ml[i][r][0]);
+  const float rref = rtop == -INFINITY ? 0.0f : rtop;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) {
+    float v[8];
+    load8(reinterpret_cast<const float*>(lds) + (i * 16 + r) * 132 + d, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += v[e];
+    lsum += ml[i][r][1] * __builtin_amdgcn_exp2f(ml[i][r][0] - rref);
+  }
+  const int rt_row = rt * 16 + r, tq = rt_row / group, hq = kvh * group + rt_row - tq * group;
+  if (p.splits == 1) {
+    const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    bf16* out = p.out + b * p.os_b + tq * p.os_n + hq * kHd + d;
+    store4(out, f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv});
+    store4(out + 4, f32x4{acc[4] * inv, acc[5] * inv, acc[6] * inv, acc[7] * inv});
+  } else {
+    const long at_row = ((static_cast<long>(b) * p.heads + hq) * p.n_q + tq) * p.splits + split;
+    store8(p.part_o + at_row * kHd + d, acc);
+    if (d == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * at_row) = f32x2{rtop, lsum};
+  }
+}
+
+// One wave per (item, head, query): lane s has split s's maximum and sum, then dims 2 l and 2 l + 1.
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs p, long total) {
+  const long row = blockIdx.x * 4L + (threadIdx.x >> 6);
+  if (row >= total) return;
+  const int lane = threadIdx.x & 63;
+  f32x2 ml = lane < p.splits ? *reinterpret_cast<const f32x2*>(p.part_ml + 2 * (row * p.splits + lane)) : f32x2{-INFINITY, 0.0f};
+  float top = ml[0];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  const float scale = __builtin_amdgcn_exp2f(ml[0] - ref);
+  const float l = wave_sum(ml[1] * scale);
+  const float* o = p.part_o + row * p.splits * kHd + 2 * lane;
+  float o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const f32x2 v = *reinterpret_cast<const f32x2*>(o + s * kHd);
+    const float f = __shfl(scale, s);
+    o0 = __builtin_fmaf(v[0], f, o0);
+    o1 = __builtin_fmaf(v[1], f, o1);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int t = static_cast<int>(row % p.n_q), h = static_cast<int>(row / p.n_q % p.heads), b = static_cast<int>(row / p.n_q / p.heads);
+  bf16* out = p.out + b * p.os_b + t * p.os_n + h * kHd + 2 * lane;
+  *reinterpret_cast<bf16x2*>(out) = bf16x2{from_f32<bf16>(o0 * inv), from_f32<bf16>(o1 * inv)};
 }
 
 // One wave per (item, head, query): lane l holds dims 2 l and 2 l + 1, one key at a time.
@@ -173,11 +672,40 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   p.scale_log2 = static_cast<float>(g.scale * 1.4426950408889634);
   return IRIS_OK;
 }
+// Which kernel a call takes, by its shapes alone.
+enum { kRows, kPrompt, kFew };
+int window_plan(WindowArgs& p) {
+  const int group = p.heads / p.kv_heads, rows = group * p.n_q;
+  if (p.ks_n >= (1L << 24) || p.vs_n >= (1L << 24)) return kRows;
+  p.hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  p.n_hgroups = group / p.hpw;
+  if (rows > 64) return kPrompt;
+  p.row_tiles = (rows + 15) / 16;
+  // keys that the last query can see at most, in tiles; splits of at least two tiles per wave that fill the CUs twice
+  long keys = p.n_k;
+  if (p.window) {
+    const long reach = (p.causal ? p.window : 2 * p.window - 1) + p.n_q - 1 + 2 * kFewKeys, sinks = p.sinks + kFewKeys;
+    keys = reach + sinks < keys ? reach + sinks : keys;
+  }
+  const long tiles = (keys + kFewKeys - 1) / kFewKeys;
+  const long base = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles;
+  long splits = (2L * device_cus() + base - 1) / base;
+  if (splits > tiles / (2 * kFewWaves)) splits = tiles / (2 * kFewWaves);
+  p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits);
+  return kFew;
+}
+long window_workspace(const WindowArgs& p) {
+  return p.splits > 1 ? static_cast<long>(p.batch) * p.heads * p.n_q * p.splits * (kHd + 2) * 4 : 0;
+}
 }  // namespace
 
 extern "C" int iris_window_attn_workspace(const iris_window_attn_args* args, long* bytes) {
-  IRIS_REQUIRE(args && bytes, "window_attn: null pointer");
+  IRIS_REQUIRE(bytes, "window_attn: null pointer");
   *bytes = 0;
+  WindowArgs p{};
+  const int rc = window_args(args, p);
+  if (rc || p.batch == 0) return rc;
+  if (window_plan(p) == kFew) *bytes = window_workspace(p);
   return IRIS_OK;
 }
 
@@ -185,8 +713,36 @@ extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t s
   WindowArgs p{};
   const int rc = window_args(args, p);
   if (rc || p.batch == 0) return rc;
-  const long total = static_cast<long>(p.batch) * p.heads * p.n_q;
-  IRIS_REQUIRE(total < (1L << 31), "window_attn: grid too large");
-  window_rows_kernel<<<dim3(static_cast<unsigned>((total + 3) / 4)), 256, 0, stream>>>(p, total);
+  const long rows = static_cast<long>(p.batch) * p.heads * p.n_q;
+  IRIS_REQUIRE(rows < (1L << 31), "window_attn: too many query rows");
+  const int plan = window_plan(p);
+  if (plan == kRows) {
+    window_rows_kernel<<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, stream>>>(p, rows);
+  } else if (plan == kPrompt) {
+    constexpr int kWaves = 4;
+    p.rows_per_wg = 32 * kWaves / p.hpw;
+    p.n_qblocks = (p.n_q + p.rows_per_wg - 1) / p.rows_per_wg;
+    const long total = static_cast<long>(p.batch) * p.kv_heads * p.n_hgroups * p.n_qblocks;
+    IRIS_REQUIRE(total < (1L << 31), "window_attn: grid too large");
+    p.total_wg = static_cast<int>(total);
+    if (p.key_mask)
+      window_attn_kernel<kWaves, 2, 64, true><<<dim3(p.total_wg), 64 * kWaves, 0, stream>>>(p);
+    else
+      window_attn_kernel<kWaves, 2, 64, false><<<dim3(p.total_wg), 64 * kWaves, 0, stream>>>(p);
+  } else {
+    const long need = window_workspace(p);
+    IRIS_REQUIRE(need == 0 || (args->workspace && aligned(args->workspace, 16) && args->workspace_bytes >= need),
+                 "window_attn: needs %ld bytes of 16-byte aligned workspace", need);
+    p.part_o = static_cast<float*>(args->workspace);
+    p.part_ml = p.part_o + rows * p.splits * kHd;
+    const long total = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles * p.splits;
+    IRIS_REQUIRE(total < (1L << 31), "window_attn: grid too large");
+    p.total_wg = static_cast<int>(total);
+    if (p.key_mask)
+      window_few_kernel<true><<<dim3(p.total_wg), 64 * kFewWaves, 0, stream>>>(p);
+    else
+      window_few_kernel<false><<<dim3(p.total_wg), 64 * kFewWaves, 0, stream>>>(p);
+    if (p.splits > 1) window_join_kernel<<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, stream>>>(p, rows);
+  }
   return check_launch("window_attn");
 }

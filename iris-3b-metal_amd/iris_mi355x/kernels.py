@@ -12,6 +12,8 @@ updates). Outputs are allocated by the wrapper unless passed in, as in the refer
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib as L
@@ -820,9 +822,16 @@ def window_attention(
     args = [q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *q_shape, *q.stride(), *k_shape, *k.stride(),
             *v.shape, *v.stride(), *place, min(window, 1 << 60), min(sinks, 1 << 60), bool(causal), lengths_at,
             lengths_kind, starts_at, starts_kind, start, mask_at, mask_stride,
-            HEAD_DIM ** -0.5 if scale is None else scale, 0, 0]
+            HEAD_DIM ** -0.5 if scale is None else scale]
     stream = _on_current_device("window_attention", q, k, v, out, lengths, starts, key_mask)
-    L.call("iris_window_attn", L.WINDOW_ATTN_ARGS.pack(*args), stream)
+    workspace = None
+    if heads * n_q <= 64 * k_shape[1]:  # few queries: their keys may be split
+        need = ctypes.c_long()
+        L.call("iris_window_attn_workspace", L.WINDOW_ATTN_ARGS.pack(*args, 0, 0), ctypes.byref(need))
+        if need.value:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            args += (workspace.data_ptr(), need.value)
+    L.call("iris_window_attn", L.WINDOW_ATTN_ARGS.pack(*args, *((0, 0) if workspace is None else ())), stream)
     return out
 
 
