@@ -18,16 +18,20 @@
 //   three rows per input row fit 16. They lie in LDS with each 8 elements in the order 0 4 1 5 2 6 3 7 that
 //   the codes come in.
 // - The FP32 sums of a group of at least 32 are scaled and added to the row's FP32 sums.
-// A workgroup's four waves take 64 NT weight rows over all of k, or, where that leaves CUs without work, 16 NT
-// rows with k dealt to the waves and their sums joined in LDS.
+// A workgroup's eight waves are dealt over weight tiles and over k (their sums joined in LDS): many tiles where
+// the weight has rows enough for all CUs, because every workgroup lays out all inputs anew, few where it has not.
 #include "iris_common.hpp"
 
 namespace iris {
 namespace {
 
-constexpr int kDepth = 4;         // code loads (16 rows x 128 k each) in flight per wave and weight tile
-constexpr int kMaxRows = 48;      // A rows of a workgroup
-constexpr int kLdsBytes = 64 << 10;  // inputs and scales of one stage of k: two workgroups per CU
+constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kMaxRows = 48;  // A rows of a workgroup
+constexpr int kAhead = 8;     // extra biases of a thread that are loaded at the start
+constexpr int kScaleItems = 8;  // scales of a thread and stage
+// LDS of a workgroup (inputs and scales of one stage of k, or of two): two workgroups per CU, or one where no CU
+// gets a second
+constexpr int kLdsTwo = 78 << 10, kLdsOne = 156 << 10;
 
 struct W4Job {
   const unsigned char* codes;
@@ -37,137 +41,253 @@ struct W4Job {
   const float *bias, *extra;
   int n_extra;
   void* out;
-  int wk;  // waves that share a weight tile's k
-  int kc;  // k per stage, a multiple of 128 wk
+  int wn;  // waves side by side over weight rows; the other kWaves / wn - 1 share their k
+  int kc;  // k per stage, a multiple of 128 kWaves / wn
 };
 struct W4Launch {
   W4Job job[2];
   int blocks0;
   const void* x;
-  int x_dtype, out_dtype, scales_dtype;
+  int out_dtype, scales_f32;
   int batch, nb;  // input rows in all, and per workgroup (blockIdx.y)
-  int parts;      // A rows per input row: 1, or 3 for FP32 and activated inputs
   int k, group, groups, in_act, out_act;
+  unsigned group_steps, group_magic;  // group / 32 and 2^32 / that + 1
 };
 
-__device__ __forceinline__ float load_any(const void* p, int dtype, long i) {
-  return dtype == IRIS_F32 ? static_cast<const float*>(p)[i] : to_f32(static_cast<const bf16*>(p)[i]);
-}
 __device__ __forceinline__ unsigned bits_of(float x) { return __builtin_bit_cast(unsigned, x); }
 __device__ __forceinline__ float of_bits(unsigned x) { return __builtin_bit_cast(float, x); }
+
+// The group of 32-wide k-step s.
+__device__ __forceinline__ int group_of(const W4Launch& a, int s) {
+  return a.group_steps == 1 ? s : static_cast<int>(__umulhi(static_cast<unsigned>(s), a.group_magic));
+}
+
+// i / d and the remainder of 0 <= i < 2^22 by d's reciprocal.
+struct Divisor {
+  int d;
+  float inv;
+  __device__ __forceinline__ explicit Divisor(int by) : d(by), inv(__builtin_amdgcn_rcpf(static_cast<float>(by))) {}
+  __device__ __forceinline__ void operator()(int i, int& q, int& r) const {
+    q = static_cast<int>(static_cast<float>(i) * inv);
+    r = i - q * d;
+    if (r < 0) --q, r += d;
+    if (r >= d) ++q, r -= d;
+  }
+};
+
+// A barrier for what passes through LDS, which leaves loads from memory underway.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // LDS of a launch: A rows of kc BF16 + 16 bytes (the 16 rows of a fragment read then start in distinct banks),
 // and per weight row and group of a stage the scale and the offset's BF16 pair, rows an odd number of pairs apart.
 __host__ __device__ __forceinline__ int x_stride(int kc) { return 2 * kc + 16; }
 __host__ __device__ __forceinline__ int stage_groups(int kc, int group) { return ((kc + group - 1) / group + 1) | 1; }
 
-// MT tiles of 16 A rows, NT of 16 weight rows per wave; SPG 32-wide k-steps per scale.
-template <int MT, int NT, int SPG>
-__global__ __launch_bounds__(256) void gemv_w4_kernel(W4Launch a) {
+// 8-element inputs of a thread and stage, by the 16-byte words that they take.
+template <typename X>
+constexpr int input_items() { return sizeof(X) == 2 ? 8 : 4; }
+
+// X: the inputs' type; PARTS: A rows per input row, 1, or 3 for FP32 and activated inputs; MT tiles of 16 A rows, NT
+// of 16 weight rows per wave; SPG 32-wide k-steps per scale; DEPTH code loads (NT of 16 rows x 128 k each) underway
+// per wave, which divides a stage's chunks of a wave where there are several stages.
+template <typename X, int PARTS, int MT, int NT, int SPG, int DEPTH>
+__global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ int odd;
+  constexpr int XI = input_items<X>();
   const bool second = static_cast<int>(blockIdx.x) >= a.blocks0;
-  const W4Job& job = second ? a.job[1] : a.job[0];
+  W4Job job = a.job[0];
+  if (second) job = a.job[1];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = 4 / job.wk, wave_n = w % wn, wave_k = w / wn;
-  const int n_wg = wn * NT * 16;
+  const int wn = job.wn, wk = kWaves / wn, wave_n = w & (wn - 1), wave_k = w / wn;
+  const int n_wg = wn * NT * 16;  // a power of two
   const int n0 = (static_cast<int>(blockIdx.x) - (second ? a.blocks0 : 0)) * n_wg;
   const int b0 = blockIdx.y * a.nb;
   const int nb = min(a.nb, a.batch - b0);
-  const int rows = nb * a.parts;
+  const int rows = nb * PARTS;
   const int k = a.k, kc = job.kc, n = job.n;
   const int xs = x_stride(kc), gs = stage_groups(kc, a.group);
-  uint2* const sc = reinterpret_cast<uint2*>(lds + a.nb * a.parts * xs);  // [n_wg][gs]
-  __shared__ unsigned bad;  // input rows (of this workgroup) with a value that is not finite
+  const int stage_bytes = a.nb * PARTS * xs + n_wg * gs * 8;  // A rows, then [n_wg][gs] scales and offsets
 
+  // codes, in chunks of 128 k dealt to the waves; past the row's end the last ones again: their inputs are zeros
   const unsigned char* codes[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
     codes[t] = job.codes + static_cast<long>(min(n0 + (wave_n * NT + t) * 16 + l16, n - 1)) * (k >> 1) + 16 * g;
-  const int chunks = (k + 127) >> 7;  // of 128 k
-  uint4 cw[kDepth][NT];
+  const int chunks = (k + 127) >> 7;
+  uint4 cw[DEPTH][NT];
   auto load = [&](int d, int c) {
+    const int at = min(c * 64, (k >> 1) - 16 - 16 * g);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-      cw[d][t] = c * 128 + 32 * g < k ? *reinterpret_cast<const uint4*>(codes[t] + 64 * static_cast<long>(c)) : uint4{0, 0, 0, 0};
+    for (int t = 0; t < NT; ++t) cw[d][t] = *reinterpret_cast<const uint4*>(codes[t] + at);
   };
-  if (tid == 0) bad = 0;
+
+  // A stage's scales and inputs: loaded into registers (while the stage before is computed), then laid out.
+  const int most_r = n - 1 - n0;
+  const char* const scale_at = static_cast<const char*>(job.scales) + static_cast<long>(n0) * a.groups * (a.scales_f32 ? 4 : 2);
+  const unsigned char* const zero_at = job.zeros + static_cast<long>(n0) * a.groups;
+  unsigned scale[kScaleItems], zero[kScaleItems];
+  auto stage_group = [&](int k0, int& g0, int& gn) {  // the first of a stage's groups and their number
+    g0 = group_of(a, k0 >> 5);
+    gn = min(group_of(a, (min(k0 + kc, k) - 1) >> 5) - g0 + 1, gs);
+  };
+  auto load_scales = [&](int k0) {
+    int g0, gn;
+    stage_group(k0, g0, gn);
+    const Divisor by_gn(gn);
+    int at[kScaleItems];
+#pragma unroll
+    for (int u = 0; u < kScaleItems; ++u) {
+      int r, q;
+      by_gn(min(tid + u * kThreads, n_wg * gn - 1), r, q);
+      at[u] = min(r, most_r) * a.groups + g0 + q;
+    }
+    if (a.scales_f32) {
+#pragma unroll
+      for (int u = 0; u < kScaleItems; ++u)
+        if (w * 64 + u * kThreads < n_wg * gn) scale[u] = *reinterpret_cast<const unsigned*>(scale_at + 4L * at[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kScaleItems; ++u)
+        if (w * 64 + u * kThreads < n_wg * gn) scale[u] = *reinterpret_cast<const unsigned short*>(scale_at + 2L * at[u]);
+    }
+    if (job.zeros) {
+#pragma unroll
+      for (int u = 0; u < kScaleItems; ++u)
+        if (w * 64 + u * kThreads < n_wg * gn) zero[u] = zero_at[at[u]];
+    }
+  };
+  auto lay_scales = [&](int k0, char* stage) {
+    uint2* const sc = reinterpret_cast<uint2*>(stage + a.nb * PARTS * xs);
+    int g0, gn;
+    stage_group(k0, g0, gn);
+    const Divisor by_gn(gn);
+#pragma unroll
+    for (int u = 0; u < kScaleItems; ++u)
+      if (w * 64 + u * kThreads < n_wg * gn) {  // (whole waves; past the last item, it again)
+        int r, q;
+        by_gn(min(tid + u * kThreads, n_wg * gn - 1), r, q);
+        // (exact: an integer below 2^8)
+        const unsigned h = bits_of(-16.0f - (job.zeros ? static_cast<float>(zero[u]) : 8.0f)) >> 16;
+        sc[r * gs + q] = uint2{a.scales_f32 ? scale[u] : scale[u] << 16, h | h << 16};
+      }
+  };
+  const int eights = kc >> 3, items = nb * eights;
+  const Divisor by_eights(eights);
+  const X* const x_at = static_cast<const X*>(a.x) + static_cast<long>(b0) * k;
+  constexpr int XW = sizeof(X) / 2;  // 16-byte words of an item
+  uint4 xr[XI][XW];
+  auto load_inputs = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < XI; ++u)
+      if (w * 64 + u * kThreads < items) {
+        int r, e;
+        by_eights(min(tid + u * kThreads, items - 1), r, e);
+        const uint4* x = reinterpret_cast<const uint4*>(x_at + r * k + min(k0 + 8 * e, k - 8));
+#pragma unroll
+        for (int i = 0; i < XW; ++i) xr[u][i] = x[i];
+      }
+  };
+  auto lay_inputs = [&](int k0, char* stage) {
+#pragma unroll
+    for (int u = 0; u < XI; ++u)
+      if (w * 64 + u * kThreads < items) {
+        int r, e;
+        by_eights(min(tid + u * kThreads, items - 1), r, e);
+        e *= 8;
+        const unsigned keep = k0 + e < k ? ~0u : 0u;
+        uint4 v = xr[u][0];
+        v = uint4{v.x & keep, v.y & keep, v.z & keep, v.w & keep};
+        if constexpr (PARTS == 1) {
+          uint4 o;
+          o.x = __builtin_amdgcn_perm(v.z, v.x, 0x05040100u);
+          o.y = __builtin_amdgcn_perm(v.z, v.x, 0x07060302u);
+          o.z = __builtin_amdgcn_perm(v.w, v.y, 0x05040100u);
+          o.w = __builtin_amdgcn_perm(v.w, v.y, 0x07060302u);
+          *reinterpret_cast<uint4*>(stage + r * xs + 2 * e) = o;
+        } else {
+          float x[8];
+          if constexpr (sizeof(X) == 4) {
+            const uint4 z = xr[u][XW - 1];
+            x[0] = of_bits(v.x), x[1] = of_bits(v.y), x[2] = of_bits(v.z), x[3] = of_bits(v.w);
+            x[4] = of_bits(z.x & keep), x[5] = of_bits(z.y & keep), x[6] = of_bits(z.z & keep), x[7] = of_bits(z.w & keep);
+          } else {
+            x[0] = of_bits(v.x << 16), x[1] = of_bits(v.x & 0xffff0000u), x[2] = of_bits(v.y << 16), x[3] = of_bits(v.y & 0xffff0000u);
+            x[4] = of_bits(v.z << 16), x[5] = of_bits(v.z & 0xffff0000u), x[6] = of_bits(v.w << 16), x[7] = of_bits(v.w & 0xffff0000u);
+          }
+          if (a.in_act == IRIS_ACT_SILU) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = silu(x[j]);  // (0 past k stays 0)
+          }
+          unsigned part[3][8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            part[0][j] = bits_of(x[j]) >> 16;
+            const float r1 = x[j] - of_bits(part[0][j] << 16);
+            part[1][j] = bits_of(r1) >> 16;
+            part[2][j] = bits_of(r1 - of_bits(part[1][j] << 16)) >> 16;
+          }
+#pragma unroll
+          for (int s = 0; s < 3; ++s)
+            *reinterpret_cast<uint4*>(stage + (s * nb + r) * xs + 2 * e) =
+                uint4{part[s][0] | part[s][4] << 16, part[s][1] | part[s][5] << 16, part[s][2] | part[s][6] << 16,
+                      part[s][3] | part[s][7] << 16};
+        }
+      }
+  };
+
+  load_scales(0);
+  load_inputs(0);
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) load(d, wave_k + d * wk);
+  // the output's row of this thread (n_wg divides the threads) and its first biases, underway from the start too
+  const int out_r = tid & (n_wg - 1), out_row = n0 + out_r, out_at = min(out_row, n - 1);
+  const int step = kThreads / n_wg, first = tid / n_wg;
+  const int outs = (job.n_extra ? job.n_extra : 1) * nb;  // (copy j, input row b), j major
+  const Divisor by_nb(nb);
+  const float bias = job.bias ? job.bias[out_at] : 0.0f;
+  float ahead[kAhead] = {};
+  if (job.n_extra) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      int j, b;
+      by_nb(min(first + u * step, outs - 1), j, b);
+      ahead[u] = job.extra[static_cast<long>(j) * n + out_at];
+    }
+  }
+  lay_scales(0, lds);
+  lay_inputs(0, lds);
+  lds_barrier();
 
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{};
-
-  const int per_stage = (kc >> 7) / job.wk;  // chunks per wave
+  // (kept in registers, one of each kind: as literals they would split every and-or in two)
+  unsigned mask = 0x00780078u, sixteen = 0x41804180u;
+  asm volatile("" : "+s"(mask), "+v"(sixteen));
+  int a_row[MT];  // LDS offset of this lane's A rows (those past the last repeat it)
+#pragma unroll
+  for (int m = 0; m < MT; ++m) a_row[m] = min(m * 16 + l16, rows - 1) * xs;
+  const int per_stage = (kc >> 7) / wk;  // chunks per wave
+  const int mine = (chunks - wave_k + wk - 1) / wk;  // of this wave in all
+  char* stage = lds;
   for (int k0 = 0, i0 = 0; k0 < k; k0 += kc, i0 += per_stage) {
-    __syncthreads();  // the last stage's reads are done (and `bad` is cleared)
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d)  // (underway while the inputs are laid out)
-      if (d < per_stage) load(d, wave_k + (i0 + d) * job.wk);
-    const int g0 = k0 / a.group;
-    // inputs: 8 elements at a time
-    const int eights = kc >> 3;
-    for (int i = tid; i < nb * eights; i += 256) {
-      const int r = i / eights, e = (i - r * eights) * 8;
-      const long at = static_cast<long>(b0 + r) * k + k0 + e;
-      const bool in = k0 + e < k;
-      if (a.parts == 1) {
-        uint4 v = in ? *reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.x) + at) : uint4{0, 0, 0, 0};
-        // not finite: an exponent of ones in either half
-        auto odd = [](unsigned u) { return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u; };
-        if (odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w)) atomicOr(&bad, 1u << (r & 31));
-        uint4 o;
-        o.x = __builtin_amdgcn_perm(v.z, v.x, 0x05040100u);
-        o.y = __builtin_amdgcn_perm(v.z, v.x, 0x07060302u);
-        o.z = __builtin_amdgcn_perm(v.w, v.y, 0x05040100u);
-        o.w = __builtin_amdgcn_perm(v.w, v.y, 0x07060302u);
-        *reinterpret_cast<uint4*>(lds + r * xs + 2 * e) = o;
-      } else {
-        float v[8];
-        if (!in) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        } else if (a.x_dtype == IRIS_F32) {
-          load8(static_cast<const float*>(a.x) + at, v);
-        } else {
-          load8(static_cast<const bf16*>(a.x) + at, v);
-        }
-        bool odd = false;
-        if (a.in_act == IRIS_ACT_SILU && in) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = silu(v[j]);
-        }
-        unsigned part[3][8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          odd |= (bits_of(v[j]) & 0x7f800000u) == 0x7f800000u;
-          part[0][j] = bits_of(v[j]) >> 16;
-          const float r1 = v[j] - of_bits(part[0][j] << 16);
-          part[1][j] = bits_of(r1) >> 16;
-          part[2][j] = bits_of(r1 - of_bits(part[1][j] << 16)) >> 16;
-        }
-        if (odd) atomicOr(&bad, 1u << (r & 31));
-#pragma unroll
-        for (int s = 0; s < 3; ++s)
-          *reinterpret_cast<uint4*>(lds + (s * nb + r) * xs + 2 * e) =
-              uint4{part[s][0] | part[s][4] << 16, part[s][1] | part[s][5] << 16, part[s][2] | part[s][6] << 16,
-                    part[s][3] | part[s][7] << 16};
-      }
+    const bool more = k0 + kc < k;
+    if (more) {
+      load_scales(k0 + kc);
+      load_inputs(k0 + kc);
     }
-    // scales and offsets of this stage's groups
-    const int gn = min((min(k0 + kc, k) - 1) / a.group - g0 + 1, gs);
-    for (int i = tid; i < n_wg * gn; i += 256) {
-      const int r = i / gn, q = i - r * gn;
-      const long at = static_cast<long>(min(n0 + r, n - 1)) * a.groups + g0 + q;
-      const float scale = load_any(job.scales, a.scales_dtype, at);
-      const float off = job.zeros ? -16.0f - static_cast<float>(job.zeros[at]) : -24.0f;
-      const unsigned h = bits_of(off) >> 16;  // (exact: an integer below 2^8)
-      sc[r * gs + q] = uint2{bits_of(scale), h | h << 16};
-    }
-    __syncthreads();
-
-    auto chunk = [&](int d, int c, bool more) {
+    const uint2* const sc = reinterpret_cast<const uint2*>(stage + a.nb * PARTS * xs);
+    int g0, gn;
+    stage_group(k0, g0, gn);
+    auto chunk = [&](int d, int c, bool next) {
       // [row][128 k] of each lane group's 32 k to [k-step of 32][lane group's 8 k]
       unsigned u[NT][4];
 #pragma unroll
@@ -178,57 +298,76 @@ __global__ __launch_bounds__(256) void gemv_w4_kernel(W4Launch a) {
         const auto s = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
         u[t][0] = r[0], u[t][1] = r[1], u[t][2] = s[0], u[t][3] = s[1];
       }
-      if (more) load(d, c + kDepth * job.wk);
+      if (next) load(d, c + DEPTH * wk);
       const int kl = c * 128 - k0;  // in the stage
+      constexpr int SG = 4 / SPG;   // scales of the chunk
+      uint2 sz[SG][NT];
 #pragma unroll
-      for (int s0 = 0; s0 < 4; s0 += SPG) {
-        const int q = (c * 128 + 32 * s0) / a.group - g0;
-        f32x4 part[MT][NT];
+      for (int q = 0; q < SG; ++q) {
+        const int at = min(group_of(a, c * 4 + SPG * q) - g0, gn - 1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sz[q][t] = sc[((wave_n * NT + t) * 16 + l16) * gs + at];
+      }
+      f32x4 part[SG][MT][NT];
+#pragma unroll
+      for (int q = 0; q < SG; ++q)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int t = 0; t < NT; ++t) part[m][t] = f32x4{};
-        uint2 sz[NT];
+          for (int t = 0; t < NT; ++t) part[q][m][t] = f32x4{};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sz[t] = sc[((wave_n * NT + t) * 16 + l16) * gs + min(q, gn - 1)];
+      for (int s = 0; s < 4; ++s) {
+        const int q = s / SPG;
+        bf16x8 af[MT];
 #pragma unroll
-        for (int s = s0; s < s0 + SPG; ++s) {
-          bf16x8 af[MT];
+        for (int m = 0; m < MT; ++m)
+          af[m] = *reinterpret_cast<const bf16x8*>(stage + a_row[m] + 2 * (kl + 32 * s + 8 * g));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const unsigned v = u[t][s], z = sz[q][t].y;
+          const uint4 b4{(v << 3 & mask) | sixteen, (v >> 1 & mask) | sixteen, (v >> 5 & mask) | sixteen,
+                         (v >> 9 & mask) | sixteen};
+          const uint4 o4{z, z, z, z};
 #pragma unroll
           for (int m = 0; m < MT; ++m)
-            af[m] = *reinterpret_cast<const bf16x8*>(lds + min(m * 16 + l16, rows - 1) * xs + 2 * (kl + 32 * s + 8 * g));
+            part[q][m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[m], __builtin_bit_cast(bf16x8, o4), part[q][m][t], 0, 0, 0);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const unsigned v = u[t][s];
-            const uint4 b4{(v << 3 & 0x00780078u) | 0x41804180u, (v >> 1 & 0x00780078u) | 0x41804180u,
-                           (v >> 5 & 0x00780078u) | 0x41804180u, (v >> 9 & 0x00780078u) | 0x41804180u};
-            const uint4 o4{sz[t].y, sz[t].y, sz[t].y, sz[t].y};
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              part[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[m], __builtin_bit_cast(bf16x8, b4), part[m][t], 0, 0, 0);
-              part[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[m], __builtin_bit_cast(bf16x8, o4), part[m][t], 0, 0, 0);
-            }
-          }
+          for (int m = 0; m < MT; ++m)
+            part[q][m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[m], __builtin_bit_cast(bf16x8, b4), part[q][m][t], 0, 0, 0);
         }
+      }
+#pragma unroll
+      for (int q = 0; q < SG; ++q)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[m][t][e] = __builtin_fmaf(of_bits(sz[t].x), part[m][t][e], acc[m][t][e]);
-      }
+            for (int e = 0; e < 4; ++e)
+              acc[m][t][e] = __builtin_fmaf(of_bits(sz[q][t].x), part[q][m][t][e], acc[m][t][e]);
+      __builtin_amdgcn_sched_barrier(0);  // (one chunk's registers at a time)
     };
-    for (int i = 0; i < per_stage; i += kDepth) {
+    // this wave's chunks of the stage; the ring's loads stand in straight code (a branch around one would wait for
+    // it) and run on into the next stage's
+    const int here = min(mine - i0, per_stage);
+    int i = 0;
+    for (; i + DEPTH <= here; i += DEPTH)
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int c = wave_k + (i0 + i + d) * job.wk;
-        if (i + d < per_stage && c < chunks) chunk(d, c, i + d + kDepth < per_stage);
-      }
+      for (int d = 0; d < DEPTH; ++d) chunk(d, wave_k + (i0 + i + d) * wk, true);
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d)
+      if (i + d < here) chunk(d, wave_k + (i0 + i + d) * wk, false);
+    if (more) {
+      stage = stage == lds ? lds + stage_bytes : lds;  // (its last readers are a barrier behind)
+      lay_scales(k0 + kc, stage);
+      lay_inputs(k0 + kc, stage);
+      lds_barrier();
     }
   }
 
   // sums to LDS: [wave_k][weight row][A row + 1]
-  __syncthreads();
+  lds_barrier();
+  if (tid == 0) odd = 0;
   float* const red = reinterpret_cast<float*>(lds);
   const int rs = MT * 16 + 1;
 #pragma unroll
@@ -238,95 +377,144 @@ __global__ __launch_bounds__(256) void gemv_w4_kernel(W4Launch a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         red[(wave_k * n_wg + (wave_n * NT + t) * 16 + l16) * rs + m * 16 + 4 * g + e] = acc[m][t][e];
-  __syncthreads();
-  // y[b][row], in place of the first wave's sums (each read and written by one thread)
-  for (int i = tid; i < nb * n_wg; i += 256) {
-    const int b = i / n_wg, r = i - b * n_wg;
+  lds_barrier();
+  // y[row][b], in place of the first wave's sums (each read and written by one thread)
+  bool finite = true;
+  for (int b = first; b < nb; b += step) {
     float y = 0.0f;
-    for (int s = a.parts - 1; s >= 0; --s)
-      for (int q = 0; q < job.wk; ++q) y += red[(q * n_wg + r) * rs + s * nb + b];
-    red[r * rs + b] = y;
+    for (int s = PARTS - 1; s >= 0; --s) {
+      float v[kWaves];
+#pragma unroll
+      for (int q = 0; q < kWaves; ++q) v[q] = red[(min(q, wk - 1) * n_wg + out_r) * rs + s * nb + b];
+#pragma unroll
+      for (int q = 0; q < kWaves; ++q) y += q < wk ? v[q] : 0.0f;
+    }
+    finite = finite && __builtin_isfinite(y);
+    red[out_r * rs + b] = y;
   }
-  __syncthreads();
-  if (bad) {  // a row holding NaN or an infinity: its products one by one, as the formula has them
-    for (int i = w; i < nb * n_wg; i += 4) {
+  if (!finite) odd = 1;
+  lds_barrier();
+  // NaN or an infinity among the inputs (or scales): the offset's products turn it into NaN, so such sums are taken
+  // product by product, as the formula has them
+  if (odd) {
+    for (int i = w; i < nb * n_wg; i += kWaves) {
       const int b = i / n_wg, r = i - b * n_wg;
-      if (!(bad >> (b & 31) & 1) || n0 + r >= n) continue;
+      if (n0 + r >= n || __builtin_isfinite(red[r * rs + b])) continue;
       const long row = n0 + r;
       float y = 0.0f;
       for (int e = lane; e < k; e += kWave) {
         const long q = row * a.groups + e / a.group;
         const unsigned code = job.codes[row * (k >> 1) + (e >> 1)] >> (4 * (e & 1)) & 15u;
-        const float wv = load_any(job.scales, a.scales_dtype, q) *
+        const float wv = (a.scales_f32 ? static_cast<const float*>(job.scales)[q] : to_f32(static_cast<const bf16*>(job.scales)[q])) *
                          (static_cast<float>(code) - (job.zeros ? static_cast<float>(job.zeros[q]) : 8.0f));
-        float xv = load_any(a.x, a.x_dtype, static_cast<long>(b0 + b) * k + e);
+        float xv = to_f32(static_cast<const X*>(a.x)[static_cast<long>(b0 + b) * k + e]);
         if (a.in_act == IRIS_ACT_SILU) xv = silu(xv);
         y = __builtin_fmaf(wv, xv, y);
       }
       y = wave_sum(y);
       if (lane == 0) red[r * rs + b] = y;
     }
-    __syncthreads();
+    lds_barrier();
   }
-  const int copies = job.n_extra ? job.n_extra : 1;
-  for (int i = tid; i < nb * n_wg; i += 256) {
-    const int b = i / n_wg, r = i - b * n_wg;
-    const int row = n0 + r;
-    if (row >= n) continue;
-    float y = red[r * rs + b];
-    if (job.bias) y += job.bias[row];
+  if (out_row >= n) return;
+  auto store = [&](long at, float v) {
+    if (a.out_dtype == IRIS_F32)
+      static_cast<float*>(job.out)[at] = v;
+    else
+      static_cast<bf16*>(job.out)[at] = from_f32<bf16>(v);
+  };
+  auto finish = [&](int i, float add) {
+    int j, b;
+    by_nb(i, j, b);
+    float y = red[out_r * rs + b];
+    if (job.bias) y += bias;
     if (a.out_act == IRIS_ACT_SILU) y = silu(y);
-    for (int j = 0; j < copies; ++j) {
-      const float v = job.n_extra ? y + job.extra[static_cast<long>(j) * n + row] : y;
-      const long at = (static_cast<long>(j) * a.batch + b0 + b) * n + row;
-      if (a.out_dtype == IRIS_F32)
-        static_cast<float*>(job.out)[at] = v;
-      else
-        static_cast<bf16*>(job.out)[at] = from_f32<bf16>(v);
-    }
-  }
+    if (job.n_extra) y += add;
+    store((static_cast<long>(j) * a.batch + b0 + b) * n + out_row, y);
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    if (first + u * step < outs) finish(first + u * step, ahead[u]);
+  for (int i = first + kAhead * step; i < outs; i += step)
+    finish(i, job.n_extra ? job.extra[static_cast<long>(i / nb) * n + out_row] : 0.0f);
 }
 
-template <int MT, int NT, int SPG>
+// One product's share of a launch: waves over weight rows and k per stage for `depth` code loads underway; 0 where
+// that depth does not fit.
+template <typename X, int PARTS, int MT, int NT>
+size_t plan_job(const W4Launch& a, W4Job& job, int& blocks, int depth) {
+  const int cus = device_cus();
+  // as many weight rows per workgroup as leave four of five CUs a workgroup (by the product's own rows, so that a
+  // result does not depend on the other product of a launch)
+  job.wn = kWaves;
+  while (job.wn > (MT > 2 ? 2 : 1) && 5L * job.n < 4L * job.wn * NT * 16 * cus) job.wn /= 2;
+  const int n_wg = job.wn * NT * 16, wk = kWaves / job.wn;
+  blocks = (job.n + n_wg - 1) / n_wg;
+  int most = blocks <= cus ? kLdsOne : kLdsTwo;
+  auto bytes = [&](int kc) { return a.nb * PARTS * x_stride(kc) + n_wg * stage_groups(kc, a.group) * 8; };
+  auto fits = [&](int kc, int stages) {
+    return a.nb * (kc / 8) <= input_items<X>() * kThreads && n_wg * stage_groups(kc, a.group) <= kScaleItems * kThreads &&
+           stages * bytes(kc) <= most;
+  };
+  const int whole = (a.k + 128 * wk - 1) / (128 * wk) * (128 * wk);
+  const size_t sums = static_cast<size_t>(wk) * n_wg * (MT * 16 + 1) * 4;
+  size_t lds;
+  if (fits(whole, 1)) {
+    job.kc = whole;
+    lds = bytes(whole);
+  } else {
+    const int unit = 128 * wk * depth;
+    if (!fits(unit, 2)) most = kLdsOne;
+    if (!fits(unit, 2)) return 0;
+    for (job.kc = unit; fits(job.kc + unit, 2);) job.kc += unit;
+    lds = 2 * static_cast<size_t>(bytes(job.kc));
+  }
+  return lds > sums ? lds : sums;
+}
+
+template <typename X, int PARTS, int MT, int NT, int SPG>
 int launch_tiles(W4Launch& a, int jobs, hipStream_t stream) {
-  // four weight tiles per workgroup where that gives every CU a workgroup, else one with k dealt to the waves
-  // (by the product's own rows, so that a result does not depend on the other product of a launch)
-  size_t lds = 0;
-  int blocks[2] = {0, 0};
-  for (int j = 0; j < jobs; ++j) {
-    W4Job& job = a.job[j];
-    job.wk = job.n >= 64L * NT * device_cus() ? 1 : 4;
-    const int n_wg = 4 / job.wk * NT * 16;
-    const int step = 128 * job.wk;
-    auto bytes = [&](int kc) { return a.nb * a.parts * x_stride(kc) + n_wg * stage_groups(kc, a.group) * 8; };
-    job.kc = (a.k + step - 1) / step * step;
-    if (bytes(job.kc) > kLdsBytes) {
-      job.kc = step;
-      while (bytes(job.kc + step) <= kLdsBytes) job.kc += step;
+  constexpr int kDepth = MT == 1 ? 4 : 2;  // (more registers spill)
+  for (int depth = kDepth; depth >= 1; depth -= kDepth - 1) {
+    size_t lds = 0;
+    int blocks[2] = {0, 0};
+    bool fit = true;
+    for (int j = 0; j < jobs; ++j) {
+      const size_t need = plan_job<X, PARTS, MT, NT>(a, a.job[j], blocks[j], depth);
+      fit = fit && need > 0;
+      lds = need > lds ? need : lds;
     }
-    const size_t need[2] = {static_cast<size_t>(bytes(job.kc)), static_cast<size_t>(job.wk) * n_wg * (MT * 16 + 1) * 4};
-    lds = need[0] > lds ? need[0] : lds;
-    lds = need[1] > lds ? need[1] : lds;
-    blocks[j] = (job.n + n_wg - 1) / n_wg;
+    if (!fit) continue;
+    a.blocks0 = blocks[0];
+    const dim3 grid(blocks[0] + blocks[1], (a.batch + a.nb - 1) / a.nb);
+    IRIS_REQUIRE(grid.y < 65536, "gemv_w4: batch too large");
+    if (depth == kDepth)
+      gemv_w4_kernel<X, PARTS, MT, NT, SPG, kDepth><<<grid, kThreads, lds, stream>>>(a);
+    else
+      gemv_w4_kernel<X, PARTS, MT, NT, SPG, 1><<<grid, kThreads, lds, stream>>>(a);
+    return check_launch("gemv_w4");
   }
-  a.blocks0 = blocks[0];
-  const dim3 grid(blocks[0] + blocks[1], (a.batch + a.nb - 1) / a.nb);
-  IRIS_REQUIRE(grid.y < 65536, "gemv_w4: batch too large");
-  gemv_w4_kernel<MT, NT, SPG><<<grid, 256, lds, stream>>>(a);
-  return check_launch("gemv_w4");
+  return fail(IRIS_E_UNSUPPORTED, "gemv_w4: no stage of k fits");  // (one of 128 k per wave always does)
 }
 
-template <int SPG>
+template <typename X, int PARTS, int SPG>
 int launch_rows(W4Launch& a, int jobs, hipStream_t stream) {
   // input rows in equal parts of at most kMaxRows A rows
-  const int most = a.parts == 1 ? 32 : kMaxRows / a.parts;
+  const int most = PARTS == 1 ? 32 : kMaxRows / PARTS;
   const int pieces = (a.batch + most - 1) / most;
   a.nb = (a.batch + pieces - 1) / pieces;
-  switch ((a.nb * a.parts + 15) / 16) {
-    case 1: return launch_tiles<1, 1, SPG>(a, jobs, stream);
-    case 2: return launch_tiles<2, 1, SPG>(a, jobs, stream);
-    default: return launch_tiles<3, 1, SPG>(a, jobs, stream);
+  switch ((a.nb * PARTS + 15) / 16) {
+    case 1: return launch_tiles<X, PARTS, 1, 1, SPG>(a, jobs, stream);
+    case 2: return launch_tiles<X, PARTS, 2, 2, SPG>(a, jobs, stream);
+    default:
+      if constexpr (PARTS == 3) return launch_tiles<X, PARTS, 3, 2, SPG>(a, jobs, stream);
+      return IRIS_E_INVALID;  // (32 rows at most)
   }
+}
+
+template <typename X, int PARTS>
+int launch_groups(W4Launch& a, int jobs, hipStream_t stream) {
+  return a.group % 64 == 0 ? launch_rows<X, PARTS, 2>(a, jobs, stream) : launch_rows<X, PARTS, 1>(a, jobs, stream);
 }
 
 }  // namespace
@@ -373,18 +561,18 @@ extern "C" int iris_gemv_w4(const iris_gemv_w4_args* args, hipStream_t stream) {
   }
   if (g.batch == 0) return IRIS_OK;
   a.x = g.x;
-  a.x_dtype = static_cast<int>(g.x_dtype);
   a.out_dtype = static_cast<int>(g.out_dtype);
-  a.scales_dtype = static_cast<int>(g.scales_dtype);
   a.batch = static_cast<int>(g.batch);
   a.k = static_cast<int>(g.k);
   a.group = static_cast<int>(g.group);
   a.groups = static_cast<int>((g.k + g.group - 1) / g.group);
+  // (k / 32 <= 2^15 and group / 32 cut to that: the product's error stays below 2^32)
+  a.group_steps = static_cast<unsigned>(g.group < (1 << 20) ? g.group / 32 : 1 << 15);
+  a.group_magic = static_cast<unsigned>((1ull << 32) / a.group_steps) + 1;
   a.in_act = static_cast<int>(g.in_act);
   a.out_act = static_cast<int>(g.out_act);
-  a.parts = a.x_dtype == IRIS_BF16 && a.in_act == IRIS_ACT_NONE ? 1 : 3;
   const int jobs = static_cast<int>(g.jobs);
-  if (a.group % 128 == 0) return launch_rows<4>(a, jobs, stream);
-  if (a.group % 64 == 0) return launch_rows<2>(a, jobs, stream);
-  return launch_rows<1>(a, jobs, stream);
+  a.scales_f32 = g.scales_dtype == IRIS_F32;
+  if (g.x_dtype == IRIS_F32) return launch_groups<float, 3>(a, jobs, stream);
+  return a.in_act == IRIS_ACT_NONE ? launch_groups<bf16, 1>(a, jobs, stream) : launch_groups<bf16, 3>(a, jobs, stream);
 }
