@@ -152,33 +152,60 @@ struct Attend {
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
-  // PARTIAL: some query may not see some key; `keys` has a bit for every key of the tile that the key mask shows.
-  template <bool PARTIAL>
-  __device__ __forceinline__ void tile(const char* kl, const char* vl, int kv0, unsigned long long keys) {
+  // partial: some query may not see some key; `keys` has a bit for every key of the tile that the key mask shows.
+  __device__ __forceinline__ void tile(const char* kl, const char* vl, int kv0, bool partial, unsigned long long keys) {
+    // S^T, the K fragments (i = NKB st + kb) read four ahead of their MFMAs; at a raised priority, so that a wave in
+    // its MFMAs is picked before those of its SIMD that are in their softmax
+    constexpr int NK = 4 * NKB;
     f32x4 s[NKB][RB];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
       for (int qb = 0; qb < RB; ++qb) s[kb][qb] = f32x4{};
+    bf16x8 kf[4];
+    auto read_k = [&](int i) { kf[i % 4] = *reinterpret_cast<const bf16x8*>(kl + (i % NKB) * 16 * 256 + k_rd[i / NKB]); };
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int st = 0; st < 4; ++st)
+    for (int i = 0; i < 4; ++i) read_k(i);
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kl + kb * 16 * 256 + k_rd[st]);
+    for (int i = 0; i < NK; ++i) {
 #pragma unroll
-        for (int qb = 0; qb < RB; ++qb)
-          s[kb][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qb][st], s[kb][qb], 0, 0, 0);
+      for (int qb = 0; qb < RB; ++qb)
+        s[i % NKB][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i % 4], qf[qb][i / NKB], s[i % NKB][qb], 0, 0, 0);
+      if (i + 4 < NK) read_k(i + 4);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads
+#pragma unroll
+    for (int i = 0; i + 4 < NK; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, RB, 0);  // MFMAs
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4 * RB, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+
+    if (partial) {
+      // (selects, not branches: the bounds of a query relative to this lane's first key)
+      const unsigned long long mine = keys >> (4 * h);
+      const unsigned bits[2] = {static_cast<unsigned>(mine), static_cast<unsigned>(mine >> 32)};
+      const int j0 = kv0 + 4 * h;
+#pragma unroll
+      for (int qb = 0; qb < RB; ++qb) {
+        const int from = j0 - span[qb].low, sinks = span[qb].sink_end - j0;
+        const unsigned width = max(span[qb].high - span[qb].low, 0);
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 16 * kb + e;
+            const int seen = (static_cast<int>(i < sinks) | static_cast<int>(static_cast<unsigned>(from + i) < width)) &
+                             static_cast<int>(bits[i / 32] >> (i % 32) & 1u);
+            s[kb][qb][e] = seen ? s[kb][qb][e] : -INFINITY;
+          }
       }
-    if constexpr (PARTIAL) {
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 16 * kb + 4 * h + e;
-#pragma unroll
-          for (int qb = 0; qb < RB; ++qb)
-            if (!visible(qb, kv0 + i, keys, i)) s[kb][qb][e] = -INFINITY;
-        }
     }
 
     // Online softmax against a running maximum that is raised lazily: while a lane's exponentials of the tile add
@@ -225,7 +252,7 @@ struct Attend {
       l[qb] += sum;
     }
 
-    if constexpr (PARTIAL) {
+    if (partial) {
       // A value that is not finite reaches every query of the MFMA (0 times NaN): where the tile holds one, it is
       // left out of the products and added to the queries that see it.
       u16x2 top{0, 0};
@@ -238,16 +265,18 @@ struct Attend {
         top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.w & 0x7fff7fffu));
       }
       if (__any(any_odd(top))) {
+#pragma unroll 1
+        for (int hf = 0; hf < H32; ++hf)
 #pragma unroll
-        for (int i = 0; i < 8 * H32; ++i) {
-          bf16x8 v = v_frag(vl, i / 8, i % 8);
+          for (int db = 0; db < 8; ++db) {
+            bf16x8 v = v_frag(vl, hf, db);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!__builtin_isfinite(to_f32(v[e]))) v[e] = from_f32<bf16>(0.0f);
+            for (int e = 0; e < 8; ++e)
+              if (!__builtin_isfinite(to_f32(v[e]))) v[e] = from_f32<bf16>(0.0f);
 #pragma unroll
-          for (int qb = 0; qb < RB; ++qb)
-            o[i % 8][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[i / 8][qb], o[i % 8][qb], 0, 0, 0);
-        }
+            for (int qb = 0; qb < RB; ++qb)
+              o[db][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, H32 == 1 || hf == 0 ? pf[0][qb] : pf[H32 - 1][qb], o[db][qb], 0, 0, 0);
+          }
 #pragma unroll 1
         for (int key = 0; key < KVT; ++key)
 #pragma unroll
@@ -263,13 +292,26 @@ struct Attend {
         return;
       }
     }
+    // O^T, the V^T fragments (i = 8 hf + db) read four ahead of their MFMAs
+    constexpr int NV = 8 * H32;
+    bf16x8 vf[4];
+    auto read_v = [&](int i) { vf[i % 4] = v_frag(vl, i / 8, i % 8); };
 #pragma unroll
-    for (int i = 0; i < 8 * H32; ++i) {
-      const bf16x8 vf = v_frag(vl, i / 8, i % 8);
+    for (int i = 0; i < 4; ++i) read_v(i);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int qb = 0; qb < RB; ++qb)
-        o[i % 8][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[i / 8][qb], o[i % 8][qb], 0, 0, 0);
+        o[i % 8][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i % 4], pf[i / 8][qb], o[i % 8][qb], 0, 0, 0);
+      if (i + 4 < NV) read_v(i + 4);
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+    for (int i = 0; i + 4 < NV; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, RB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4 * RB, 0);
   }
 };
 
@@ -389,10 +431,7 @@ window_attn_kernel(WindowArgs p) {
     constexpr unsigned long long kAll = KVT == 64 ? ~0ull : (1ull << (KVT & 63)) - 1;
     if (MASK && !(keys & kAll)) continue;
     const char* kl = lds + stage * STAGE;
-    if (sees_all<KVT>(first, last, kv0) && (!MASK || (keys & kAll) == kAll))
-      at.template tile<false>(kl, kl + KVT * 256, kv0, keys);
-    else
-      at.template tile<true>(kl, kl + KVT * 256, kv0, keys);
+    at.tile(kl, kl + KVT * 256, kv0, !sees_all<KVT>(first, last, kv0) || (MASK && (keys & kAll) != kAll), keys);
   }
 
 #pragma unroll
@@ -482,10 +521,7 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
     constexpr unsigned long long kAll = (1ull << KVT) - 1;
     if (MASK && !(keys & kAll)) continue;
     const char* kl = mine + stage * STAGE;
-    if (sees_all<KVT>(first, last, kv0) && (!MASK || (keys & kAll) == kAll))
-      at.template tile<false>(kl, kl + KVT * 256, kv0, keys);
-    else
-      at.template tile<true>(kl, kl + KVT * 256, kv0, keys);
+    at.tile(kl, kl + KVT * 256, kv0, !sees_all<KVT>(first, last, kv0) || (MASK && (keys & kAll) != kAll), keys);
   }
 
   // join the waves: every wave's sums against the largest of their maxima, then one thread per 8 dims of a row
