@@ -21,6 +21,8 @@
 // window_rows_kernel: row strides too large for the 32-bit offsets of the others.
 #include "iris_common.hpp"
 
+#include <type_traits>
+
 namespace iris {
 namespace {
 
@@ -46,7 +48,6 @@ struct WindowArgs {
 };
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 __host__ __device__ __forceinline__ long clamp_long(long x, long lo, long hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
@@ -83,6 +84,13 @@ __device__ __forceinline__ void wait_vmcnt() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
 
+// A barrier for what passes through LDS, which leaves loads from memory underway.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Lane i of 16 gets column i of the 4 x 16 block whose row j the lanes 4 j .. 4 j + 3 address, 8 bytes each.
 __device__ __forceinline__ bf16x4 read_tr(const char* p) {
   return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
@@ -101,12 +109,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const bf16* p, lon
 __device__ __forceinline__ int k_swz(int row) { return row & 15; }
 __device__ __forceinline__ int v_swz(int row) { return 2 * (row & 7); }
 
-__device__ __forceinline__ bool any_odd(u16x2 top) { return top[0] >= 0x7f80 || top[1] >= 0x7f80; }
-
-// The running attention of 16 RB queries of one head per wave over tiles of KVT keys in LDS (K rows, then V rows,
-// 256 bytes each). Lane l (l16 = l % 16, h = l / 16) owns queries 16 qb + l16 and, of each 16 keys of a tile, keys
-// 4 h .. 4 h + 3: s[kb][qb][e] is key 16 kb + 4 h + e. The keys of a P V step (32 of them) are taken in the order
-// 16 (j / 4) + 4 h + j % 4 for k-index 8 h + j, in P^T and V^T alike. o[db][qb][e] is dim 16 db + 4 h + e.
+// The running attention of 16 RB queries of one head per wave over tiles of KVT keys in LDS (K rows, V rows, 256 bytes
+// each). Lane l (l16 = l % 16, h = l / 16) owns queries 16 qb + l16 and, of each 16 keys, keys 4 h .. 4 h + 3:
+// s[kb][qb][e] is key 16 kb + 4 h + e. A P V step of 32 keys takes them in the order 16 (j / 4) + 4 h + j % 4 for
+// k-index 8 h + j, in P^T and V^T alike. o[db][qb][e] is dim 16 db + 4 h + e.
 template <int RB, int KVT>
 struct Attend {
   static constexpr int NKB = KVT / 16, H32 = KVT / 32;
@@ -114,7 +120,7 @@ struct Attend {
   f32x4 o[8][RB];
   float m[RB], l[RB];  // log2 domain; l: this lane's keys only
   Span span[RB];
-  int k_rd[4], v_rd[8];
+  int k_rd[4], v_rd[8];  // LDS offsets of the fragment reads by k-step and dim block
   int l16, h;
   float sl2;  // > 0
 
@@ -132,57 +138,84 @@ struct Attend {
   __device__ __forceinline__ void start(int lane) {
     l16 = lane & 15, h = lane >> 4;
 #pragma unroll
-    for (int qb = 0; qb < RB; ++qb) m[qb] = -INFINITY, l[qb] = 0.0f;
-#pragma unroll
-    for (int db = 0; db < 8; ++db)
-#pragma unroll
-      for (int qb = 0; qb < RB; ++qb) o[db][qb] = f32x4{};
-#pragma unroll
     for (int st = 0; st < 4; ++st) k_rd[st] = l16 * 256 + 16 * ((4 * st + h) ^ k_swz(l16));
     const int row = 4 * h + (l16 >> 2);
 #pragma unroll
     for (int db = 0; db < 8; ++db)
       v_rd[db] = row * 256 + 16 * ((2 * db + ((l16 & 3) >> 1)) ^ v_swz(row)) + 8 * (l16 & 1);
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int qb = 0; qb < RB; ++qb) m[qb] = -INFINITY, l[qb] = 0.0f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+#pragma unroll
+      for (int qb = 0; qb < RB; ++qb) o[db][qb] = f32x4{};
+  }
+  // Whether some output is not finite.
+  __device__ __forceinline__ bool odd() const {
+    float x = 0.0f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+#pragma unroll
+      for (int qb = 0; qb < RB; ++qb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = __builtin_fmaf(o[db][qb][e], 0.0f, x);
+    return x != 0.0f;  // (NaN)
   }
   __device__ __forceinline__ bool visible(int qb, int j, unsigned long long keys, int in_tile) const {
     return (j < span[qb].sink_end || (j >= span[qb].low && j < span[qb].high)) && (keys >> in_tile & 1);
   }
   __device__ __forceinline__ bf16x8 v_frag(const char* vl, int hf, int db) const {
-    const bf16x4 a = read_tr(vl + hf * 32 * 256 + v_rd[db]), b = read_tr(vl + (hf * 32 + 16) * 256 + v_rd[db]);
+    const char* p = vl + hf * 32 * 256 + v_rd[db];
+    const bf16x4 a = read_tr(p), b = read_tr(p + 16 * 256);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
   // partial: some query may not see some key; `keys` has a bit for every key of the tile that the key mask shows.
-  __device__ __forceinline__ void tile(const char* kl, const char* vl, int kv0, bool partial, unsigned long long keys) {
-    // S^T, the K fragments (i = NKB st + kb) read four ahead of their MFMAs; at a raised priority, so that a wave in
-    // its MFMAs is picked before those of its SIMD that are in their softmax
+  // careful: values that are not finite may be among the tile's.
+  // K: the tile's K rows in LDS, or its K fragments (i = NKB st + kb) in registers.
+  template <typename K>
+  __device__ __forceinline__ void tile(K kl, const char* vl, int kv0, bool partial, unsigned long long keys, bool careful) {
+    // S^T, K fragments from LDS read four ahead of their MFMAs; at a raised priority, so that a wave in its MFMAs is
+    // picked before those of its SIMD that are in their softmax
     constexpr int NK = 4 * NKB;
+    constexpr bool kLds = std::is_same<K, const char*>::value;
     f32x4 s[NKB][RB];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
       for (int qb = 0; qb < RB; ++qb) s[kb][qb] = f32x4{};
-    bf16x8 kf[4];
-    auto read_k = [&](int i) { kf[i % 4] = *reinterpret_cast<const bf16x8*>(kl + (i % NKB) * 16 * 256 + k_rd[i / NKB]); };
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kLds) {
+      bf16x8 kf[4];
+      auto read_k = [&](int i) { kf[i % 4] = *reinterpret_cast<const bf16x8*>(kl + (i % NKB) * 16 * 256 + k_rd[i / NKB]); };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) read_k(i);
+      for (int i = 0; i < 4; ++i) read_k(i);
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
+      for (int i = 0; i < NK; ++i) {
 #pragma unroll
-      for (int qb = 0; qb < RB; ++qb)
-        s[i % NKB][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i % 4], qf[qb][i / NKB], s[i % NKB][qb], 0, 0, 0);
-      if (i + 4 < NK) read_k(i + 4);
+        for (int qb = 0; qb < RB; ++qb)
+          s[i % NKB][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i % 4], qf[qb][i / NKB], s[i % NKB][qb], 0, 0, 0);
+        if (i + 4 < NK) read_k(i + 4);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads
+#pragma unroll
+      for (int i = 0; i + 4 < NK; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, RB, 0);  // MFMAs
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4 * RB, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int qb = 0; qb < RB; ++qb)
+          s[i % NKB][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kl[i], qf[qb][i / NKB], s[i % NKB][qb], 0, 0, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads
-#pragma unroll
-    for (int i = 0; i + 4 < NK; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, RB, 0);  // MFMAs
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4 * RB, 0);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
@@ -251,46 +284,33 @@ struct Attend {
       }
       l[qb] += sum;
     }
-
-    if (partial) {
-      // A value that is not finite reaches every query of the MFMA (0 times NaN): where the tile holds one, it is
-      // left out of the products and added to the queries that see it.
-      u16x2 top{0, 0};
+    if (careful) {
+      // A value that is not finite reaches every query of the MFMA (0 times NaN): where some query does not see the
+      // tile whole, it is left out of the products and added to the queries that see it.
 #pragma unroll
       for (int i = 0; i < 8 * H32; ++i) {
-        const uint4 v = __builtin_bit_cast(uint4, v_frag(vl, i / 8, i % 8));
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.x & 0x7fff7fffu));
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.y & 0x7fff7fffu));
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.z & 0x7fff7fffu));
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v.w & 0x7fff7fffu));
+        bf16x8 v = v_frag(vl, i / 8, i % 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (partial && !__builtin_isfinite(to_f32(v[e]))) v[e] = from_f32<bf16>(0.0f);
+#pragma unroll
+        for (int qb = 0; qb < RB; ++qb)
+          o[i % 8][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pf[i / 8][qb], o[i % 8][qb], 0, 0, 0);
       }
-      if (__any(any_odd(top))) {
+      if (!partial) return;
 #pragma unroll 1
-        for (int hf = 0; hf < H32; ++hf)
+      for (int key = 0; key < KVT; ++key)
 #pragma unroll
-          for (int db = 0; db < 8; ++db) {
-            bf16x8 v = v_frag(vl, hf, db);
+        for (int db = 0; db < 8; ++db) {
+          const int d = 16 * db + 4 * h;
+          const f32x4 v = load4(reinterpret_cast<const bf16*>(vl + key * 256 + 16 * ((d >> 3) ^ v_swz(key)) + 2 * (d & 7)));
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (!__builtin_isfinite(to_f32(v[e]))) v[e] = from_f32<bf16>(0.0f);
+          for (int qb = 0; qb < RB; ++qb)
 #pragma unroll
-            for (int qb = 0; qb < RB; ++qb)
-              o[db][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, H32 == 1 || hf == 0 ? pf[0][qb] : pf[H32 - 1][qb], o[db][qb], 0, 0, 0);
-          }
-#pragma unroll 1
-        for (int key = 0; key < KVT; ++key)
-#pragma unroll
-          for (int db = 0; db < 8; ++db) {
-            const int d = 16 * db + 4 * h;
-            const f32x4 v = load4(reinterpret_cast<const bf16*>(vl + key * 256 + 16 * ((d >> 3) ^ v_swz(key)) + 2 * (d & 7)));
-#pragma unroll
-            for (int qb = 0; qb < RB; ++qb)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!__builtin_isfinite(v[e]) && visible(qb, kv0 + key, keys, key)) o[db][qb][e] += v[e];
-          }
-        return;
-      }
+            for (int e = 0; e < 4; ++e)
+              if (!__builtin_isfinite(v[e]) && visible(qb, kv0 + key, keys, key)) o[db][qb][e] += v[e];
+        }
+      return;
     }
     // O^T, the V^T fragments (i = 8 hf + db) read four ahead of their MFMAs
     constexpr int NV = 8 * H32;
@@ -313,6 +333,18 @@ struct Attend {
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 4 * RB, 0);
   }
+
+  // A tile, if some query between those of the spans a and z sees a key of it.
+  template <bool MASK, typename K>
+  __device__ __forceinline__ void visit(const Span& a, const Span& z, K kl, const char* vl, int kv0,
+                                        unsigned long long keys, bool careful) {
+    constexpr unsigned long long kAll = KVT == 64 ? ~0ull : (1ull << (KVT & 63)) - 1;
+    // (none of it: below the windows and past the first keys, or past the windows)
+    if (kv0 >= z.sink_end && (kv0 >= z.high || kv0 + KVT <= a.low)) return;
+    if (MASK && !(keys & kAll)) return;
+    const bool all = kv0 + KVT <= a.sink_end || (kv0 >= z.low && kv0 + KVT <= a.high);
+    tile(kl, vl, kv0, !all || (MASK && (keys & kAll) != kAll), keys, careful);
+  }
 };
 
 // The tiles that hold a visible key of queries at positions first .. last: those of [0, sinks), then those of
@@ -329,28 +361,20 @@ struct Tiles {
   }
   __device__ __forceinline__ int key(int t) const { return (t < sink ? t : t - sink + band) * KVT; }
 };
-// Whether queries at positions with the spans a (the first) .. z (the last) see all, or none, of a tile.
-template <int KVT>
-__device__ __forceinline__ bool sees_all(const Span& a, const Span& z, int kv0) {
-  return kv0 + KVT <= a.sink_end || (kv0 >= z.low && kv0 + KVT <= a.high);
-}
-template <int KVT>
-__device__ __forceinline__ bool sees_none(const Span& a, const Span& z, int kv0) {
-  return kv0 >= z.sink_end && (kv0 >= z.high || kv0 + KVT <= a.low);
-}
-
 // A bit for every key of the tile at kv0 that the mask shows, from one byte per lane.
 __device__ __forceinline__ int mask_byte(const unsigned char* mask, int kv0, int lane, int length) {
   return kv0 + lane < length ? mask[kv0 + lane] : 0;
 }
 
-template <int NW, int STAGES, int KVT, bool MASK>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 12 ? 3 : 2))) void
+template <int RB, int NW, int STAGES, int KVT, bool MASK>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void
 window_attn_kernel(WindowArgs p) {
   constexpr int STAGE = 2 * KVT * 256;  // bytes: K rows, then V rows
   constexpr int LOADS = KVT / 16;       // 1 KB loads (4 rows) per fetching wave and operand; the first four waves fetch
   constexpr int LPW = 2 * LOADS;
   static_assert((KVT == 32 || KVT == 64) && STAGES >= 2 && (STAGES - 2) * LPW < 64, "pipeline");
+  // (the only LDS of the kernel: with a second object, a fence's included, the compiler waits for the prefetch before
+  // every tile's reads)
   __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
 
   // logical workgroup: (item, K/V head, head group) major, query block minor and, where later queries see more
@@ -370,18 +394,18 @@ window_attn_kernel(WindowArgs p) {
   const int length = __builtin_amdgcn_readfirstlane(item_length(p, b));
   const long pos0 = item_start(p, b, length);
   const int wg0 = qblk * p.rows_per_wg;
-  const int q0 = wg0 + (w / p.hpw) * 32;
+  const int q0 = wg0 + (w / p.hpw) * 16 * RB;
 
-  Attend<2, KVT> at;
+  Attend<RB, KVT> at;
   at.start(lane);
 #pragma unroll
-  for (int qb = 0; qb < 2; ++qb) {
+  for (int qb = 0; qb < RB; ++qb) {
     const int row = min(q0 + 16 * qb + at.l16, p.n_q - 1);
     at.load_query(qb, p.q + b * p.qs_b + hd * p.qs_h + row * p.qs_n, p.scale_log2);
     at.span[qb] = span_of(p, pos0 + row, length);
   }
   const Tiles<KVT> tiles(p, pos0 + wg0, pos0 + min(wg0 + p.rows_per_wg, p.n_q) - 1, length);
-  const Span first = span_of(p, pos0 + min(q0, p.n_q - 1), length), last = span_of(p, pos0 + min(q0 + 31, p.n_q - 1), length);
+  const Span first = span_of(p, pos0 + min(q0, p.n_q - 1), length), last = span_of(p, pos0 + min(q0 + 16 * RB - 1, p.n_q - 1), length);
   const bool idle = q0 >= p.n_q;
 
   const bf16* kh = p.k + b * p.ks_b + kvh * p.ks_h;
@@ -394,48 +418,71 @@ window_attn_kernel(WindowArgs p) {
     k_off[j] = r * static_cast<int>(p.ks_n) * 2 + 16 * ((lane & 15) ^ k_swz(r));
     v_off[j] = r * static_cast<int>(p.vs_n) * 2 + 16 * ((lane & 15) ^ v_swz(r));
   }
+  const __amdgpu_buffer_rsrc_t rk = rows_buffer(kh, length, p.ks_n), rv = rows_buffer(vh, length, p.vs_n);
   auto issue = [&](int t, int stage) {
     if (NW != 4 && w >= 4) return;
     const int kv0 = tiles.key(t);
-    const __amdgpu_buffer_rsrc_t rk = rows_buffer(kh + kv0 * p.ks_n, length - kv0, p.ks_n);
-    const __amdgpu_buffer_rsrc_t rv = rows_buffer(vh + kv0 * p.vs_n, length - kv0, p.vs_n);
+    const int ks = kv0 * static_cast<int>(p.ks_n) * 2, vs = kv0 * static_cast<int>(p.vs_n) * 2;
     bf16* kl = reinterpret_cast<bf16*>(lds + stage * STAGE);
     bf16* vl = kl + KVT * kHd;
+    if (kv0 + KVT <= length) {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      buffer_load_lds16(rk, kl + (w * LOADS + j) * 512, k_off[j], 0);
-      buffer_load_lds16(rv, vl + (w * LOADS + j) * 512, v_off[j], 0);
+      for (int j = 0; j < LOADS; ++j) {
+        buffer_load_lds16(rk, kl + (w * LOADS + j) * 512, k_off[j], ks);
+        buffer_load_lds16(rv, vl + (w * LOADS + j) * 512, v_off[j], vs);
+      }
+    } else {  // the last key again in the rows past it
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int r = (w * LOADS + j) * 4 + (lane >> 4), back = max(r - (length - 1 - kv0), 0);
+        buffer_load_lds16(rk, kl + (w * LOADS + j) * 512, k_off[j] - back * static_cast<int>(p.ks_n) * 2, ks);
+        buffer_load_lds16(rv, vl + (w * LOADS + j) * 512, v_off[j] - back * static_cast<int>(p.vs_n) * 2, vs);
+      }
     }
   };
 
   const int n_tiles = tiles.count;
-  int byte = MASK && n_tiles > 0 ? mask_byte(mask, tiles.key(0), lane, length) : 0;
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (s < n_tiles) issue(s, s);
-  for (int t = 0, stage = 0; t < n_tiles; ++t, stage = stage + 1 == STAGES ? 0 : stage + 1) {
-    unsigned long long keys = ~0ull;
-    if (MASK) {
-      keys = __ballot(byte != 0);
-      if (t + 1 < n_tiles) byte = mask_byte(mask, tiles.key(t + 1), lane, length);
+  for (int pass = 0; pass < 2; ++pass) {
+    int byte = MASK && n_tiles > 0 ? mask_byte(mask, tiles.key(0), lane, length) : 0;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < n_tiles) issue(s, s);
+    for (int t = 0, stage = 0; t < n_tiles; ++t, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+      unsigned long long keys = ~0ull;
+      if (MASK) {
+        keys = __ballot(byte != 0);
+        if (t + 1 < n_tiles) byte = mask_byte(mask, tiles.key(t + 1), lane, length);
+      }
+      if (t + STAGES - 2 < n_tiles)
+        wait_vmcnt<(STAGES - 2) * LPW>();
+      else
+        wait_vmcnt<0>();
+      __builtin_amdgcn_s_barrier();  // tile t is there; the stage of tile t - 1 is no longer read
+      asm volatile("" ::: "memory");
+      if (t + STAGES - 1 < n_tiles) issue(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+      const int kv0 = tiles.key(t);
+      if (idle) continue;
+      const char* kl = lds + stage * STAGE;
+      at.template visit<MASK>(first, last, kl, kl + KVT * 256, kv0, keys, pass != 0);
     }
-    if (t + STAGES - 2 < n_tiles)
-      wait_vmcnt<(STAGES - 2) * LPW>();
-    else
-      wait_vmcnt<0>();
-    __builtin_amdgcn_s_barrier();  // tile t is there; the stage of tile t - 1 is no longer read
-    asm volatile("" ::: "memory");
-    if (t + STAGES - 1 < n_tiles) issue(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-    const int kv0 = tiles.key(t);
-    if (idle || sees_none<KVT>(first, last, kv0)) continue;
-    constexpr unsigned long long kAll = KVT == 64 ? ~0ull : (1ull << (KVT & 63)) - 1;
-    if (MASK && !(keys & kAll)) continue;
-    const char* kl = lds + stage * STAGE;
-    at.tile(kl, kl + KVT * 256, kv0, !sees_all<KVT>(first, last, kv0) || (MASK && (keys & kAll) != kAll), keys);
+    // not finite: once more, keeping such values to the queries that see them
+    if (pass == 1) break;
+    int* const flags = reinterpret_cast<int*>(lds);
+    lds_barrier();  // (the last tile is read)
+    if (lane == 0) flags[w] = 0;
+    if (at.odd()) flags[w] = 1;
+    lds_barrier();
+    int odd = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) odd |= flags[i];
+    if (!odd) break;
+    lds_barrier();
+    at.clear();
   }
 
 #pragma unroll
-  for (int qb = 0; qb < 2; ++qb) {
+  for (int qb = 0; qb < RB; ++qb) {
     float l = at.l[qb] + __shfl_xor(at.l[qb], 16);
     l += __shfl_xor(l, 32);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -447,15 +494,23 @@ window_attn_kernel(WindowArgs p) {
   }
 }
 
-// Few queries: the 16 rows of a wave's tile are (query, head of the group) pairs r = t group + g of one K/V head.
-constexpr int kFewWaves = 4, kFewKeys = 32, kFewStages = 2;
+// Few queries: the 16 rows of a wave's tile are (query, head of the group) pairs r = t group + g of one K/V head. K
+// fragments go straight to registers (a lane's row of 16 keys), V rows to the wave's ring in LDS.
+constexpr int kFewWaves = 8, kFewKeys = 32;
 constexpr int kMaxSplits = 64;
 
+// Tiles of a split: whole rounds of the waves.
+__host__ __device__ __forceinline__ int few_share(int tiles, int splits) {
+  return (tiles + splits * kFewWaves - 1) / (splits * kFewWaves) * kFewWaves;
+}
+
 template <bool MASK>
-__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(1))) void window_few_kernel(WindowArgs p) {
-  constexpr int KVT = kFewKeys, STAGE = 2 * KVT * 256, LOADS = KVT / 4, LPW = 2 * LOADS;
-  __shared__ __attribute__((aligned(1024))) char lds[kFewWaves * kFewStages * STAGE];
-  __shared__ float ml[kFewWaves][16][2];
+__global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(2))) void window_few_kernel(WindowArgs p) {
+  constexpr int KVT = kFewKeys, STAGE = KVT * 256, LOADS = KVT / 4;
+  // (one object, as in window_attn_kernel: the V rings, two stages a wave; after the loop the waves' sums, then their
+  // maxima)
+  __shared__ __attribute__((aligned(1024))) char lds[kFewWaves * 2 * STAGE];
+  float (*const ml)[16][2] = reinterpret_cast<float (*)[16][2]>(lds + kFewWaves * 16 * 132 * 4);
 
   int wg = xcd_remap(blockIdx.x, p.total_wg);
   const int rt = wg % p.row_tiles;
@@ -469,66 +524,76 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
   const int group = p.heads / p.kv_heads, rows = group * p.n_q;
   const int length = __builtin_amdgcn_readfirstlane(item_length(p, b));
   const long pos0 = item_start(p, b, length);
-
-  Attend<1, KVT> at;
-  at.start(lane);
-  const int row = min(rt * 16 + at.l16, rows - 1), t_row = row / group, hd = kvh * group + row - t_row * group;
-  at.load_query(0, p.q + b * p.qs_b + hd * p.qs_h + t_row * p.qs_n, p.scale_log2);
-  at.span[0] = span_of(p, pos0 + t_row, length);
   const long pos_a = pos0 + rt * 16 / group, pos_z = pos0 + min(rt * 16 + 15, rows - 1) / group;
   const Span first = span_of(p, pos_a, length), last = span_of(p, pos_z, length);
   const Tiles<KVT> tiles(p, pos_a, pos_z, length);
-  const int per = (tiles.count + p.splits - 1) / p.splits;
-  const int end = min(tiles.count, (split + 1) * per);
+  const int per = few_share(tiles.count, p.splits);
+  const int t0 = split * per + w, end = min(tiles.count, (split + 1) * per);
 
   const bf16* kh = p.k + b * p.ks_b + kvh * p.ks_h;
   const bf16* vh = p.v + b * p.vs_b + kvh * p.vs_h;
   const unsigned char* mask = MASK ? p.key_mask + b * p.mask_stride : nullptr;
-  int k_off[LOADS], v_off[LOADS];
+  Attend<1, KVT> at;
+  at.start(lane);
+  const int k_off = at.l16 * static_cast<int>(p.ks_n) * 2 + 16 * at.h;  // (a fragment: row l16 of 16 keys, 8 dims)
+  int v_off[LOADS];
 #pragma unroll
   for (int j = 0; j < LOADS; ++j) {
     const int r = j * 4 + (lane >> 4);
-    k_off[j] = r * static_cast<int>(p.ks_n) * 2 + 16 * ((lane & 15) ^ k_swz(r));
     v_off[j] = r * static_cast<int>(p.vs_n) * 2 + 16 * ((lane & 15) ^ v_swz(r));
   }
-  char* const mine = lds + w * kFewStages * STAGE;
+  char* const mine = lds + w * 2 * STAGE;
+  bf16x8 kf[2][8];
+  int byte[2];
+  // (STAGE-constant: the registers of the two stages; the K loads first, so that they are waited for alone)
   auto issue = [&](int t, int stage) {
     const int kv0 = tiles.key(t);
     const __amdgpu_buffer_rsrc_t rk = rows_buffer(kh + kv0 * p.ks_n, length - kv0, p.ks_n);
     const __amdgpu_buffer_rsrc_t rv = rows_buffer(vh + kv0 * p.vs_n, length - kv0, p.vs_n);
-    bf16* kl = reinterpret_cast<bf16*>(mine + stage * STAGE);
+    const int half = 16 * static_cast<int>(p.ks_n) * 2;
+    if (MASK) byte[stage] = mask_byte(mask, kv0, lane, length);
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) buffer_load_lds16(rk, kl + j * 512, k_off[j], 0);
+    for (int i = 0; i < 8; ++i)
+      kf[stage][i] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off + 64 * (i / 2) + (i % 2) * half, 0, 0));
+    bf16* vl = reinterpret_cast<bf16*>(mine + stage * STAGE);
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) buffer_load_lds16(rv, kl + KVT * kHd + j * 512, v_off[j], 0);
+    for (int j = 0; j < LOADS; ++j) buffer_load_lds16(rv, vl + j * 512, v_off[j], 0);
   };
-  int t = split * per + w;
-  int byte = MASK && t < end ? mask_byte(mask, tiles.key(t), lane, length) : 0;
-  if (t < end) issue(t, 0);
-  for (int stage = 0; t < end; t += kFewWaves, stage ^= 1) {
-    unsigned long long keys = ~0ull;
-    if (MASK) keys = __ballot(byte != 0);
-    if (t + kFewWaves < end) {
-      if (MASK) byte = mask_byte(mask, tiles.key(t + kFewWaves), lane, length);
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage's last reads are done
-      issue(t + kFewWaves, stage ^ 1);
-      wait_vmcnt<LPW>();
-    } else {
-      wait_vmcnt<0>();
+  if (t0 < end) issue(t0, 0);
+  const int row = min(rt * 16 + at.l16, rows - 1), t_row = row / group, hd = kvh * group + row - t_row * group;
+  at.load_query(0, p.q + b * p.qs_b + hd * p.qs_h + t_row * p.qs_n, p.scale_log2);
+  at.span[0] = span_of(p, pos0 + t_row, length);
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1 && t0 < end) issue(t0, 0);
+    for (int t = t0; t < end;) {
+#pragma unroll
+      for (int stage = 0; stage < 2; ++stage) {
+        if (t >= end) break;
+        if (t + kFewWaves < end) {
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the other stage's last reads are done
+          issue(t + kFewWaves, stage ^ 1);
+          wait_vmcnt<8 + LOADS>();
+        } else {
+          wait_vmcnt<0>();
+        }
+        asm volatile("" ::: "memory");
+        const unsigned long long keys = MASK ? __ballot(byte[stage] != 0) : ~0ull;
+        at.template visit<MASK>(first, last, &kf[stage][0], mine + stage * STAGE, tiles.key(t), keys, pass != 0);
+        t += kFewWaves;
+      }
     }
-    asm volatile("" ::: "memory");
-    const int kv0 = tiles.key(t);
-    constexpr unsigned long long kAll = (1ull << KVT) - 1;
-    if (MASK && !(keys & kAll)) continue;
-    const char* kl = mine + stage * STAGE;
-    at.tile(kl, kl + KVT * 256, kv0, !sees_all<KVT>(first, last, kv0) || (MASK && (keys & kAll) != kAll), keys);
+    if (pass == 1 || !__any(at.odd())) break;  // as in window_attn_kernel, each wave for itself
+    at.clear();
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   }
 
   // join the waves: every wave's sums against the largest of their maxima, then one thread per 8 dims of a row
   float l = at.l[0] + __shfl_xor(at.l[0], 16);
   l += __shfl_xor(l, 32);
+  lds_barrier();  // (the rings are no longer read)
   if (lane < 16) ml[w][lane][0] = at.m[0], ml[w][lane][1] = l;
-  __syncthreads();  // (the rings are no longer read)
+  lds_barrier();
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kFewWaves; ++i) top = fmaxf(top, ml[i][at.l16][0]);
@@ -537,9 +602,9 @@ __global__ __launch_bounds__(64 * kFewWaves) __attribute__((amdgpu_waves_per_eu(
   float* const sums = reinterpret_cast<float*>(lds) + w * 16 * 132;  // rows of 132: distinct banks
 #pragma unroll
   for (int db = 0; db < 8; ++db) store4(sums + at.l16 * 132 + 16 * db + 4 * at.h, at.o[db][0] * mine_scale);
-  __syncthreads();
+  lds_barrier();
   const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
-  if (rt * 16 + r >= rows) return;
+  if (r >= 16 || rt * 16 + r >= rows) return;
   float acc[8] = {}, lsum = 0.0f, rtop = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kFewWaves; ++i) rtop = fmaxf(rtop, ml[i][r][0]);
@@ -712,22 +777,31 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
 enum { kRows, kPrompt, kFew };
 int window_plan(WindowArgs& p) {
   const int group = p.heads / p.kv_heads, rows = group * p.n_q;
-  if (p.ks_n >= (1L << 24) || p.vs_n >= (1L << 24)) return kRows;
+  if (p.ks_n >= (1L << 24) || p.vs_n >= (1L << 24)) return kRows;  // (32 rows of a tile by 32-bit offsets)
   p.hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
   p.n_hgroups = group / p.hpw;
-  if (rows > 64) return kPrompt;
+  if (rows > 64)  // (all rows by 32-bit offsets)
+    return (p.n_k + 64) * (p.ks_n > p.vs_n ? p.ks_n : p.vs_n) * 2 < (1L << 31) ? kPrompt : kRows;
   p.row_tiles = (rows + 15) / 16;
-  // keys that the last query can see at most, in tiles; splits of at least two tiles per wave that fill the CUs twice
+  // keys that the queries can see at most, in tiles
   long keys = p.n_k;
   if (p.window) {
     const long reach = (p.causal ? p.window : 2 * p.window - 1) + p.n_q - 1 + 2 * kFewKeys, sinks = p.sinks + kFewKeys;
     keys = reach + sinks < keys ? reach + sinks : keys;
   }
+  // a workgroup for every CU, of one tile a wave at least; where every wave keeps 16 tiles, up to four for every CU.
+  // us by the number of splits: one token, 20 on 5 heads, 1028 keys 1: 15.2, 4: 11.4, 8: 11.5, 16: 13.1; 4096 keys
+  // 4: 20.4, 8: 16.0, 16: 15.6, 32: 17.7; 16384 keys 8: 32.6, 16: 24.6, 32: 22.9; 32 on 8 heads, 65536 keys 16: 82,
+  // 32: 66, 64: 76; 16 items of 4096 keys 1: 76, 2: 59, 4: 59, 8: 65; of 65536 keys 1: 1077, 2: 781, 4: 749, 8: 727
   const long tiles = (keys + kFewKeys - 1) / kFewKeys;
-  const long base = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles;
-  long splits = (2L * device_cus() + base - 1) / base;
-  if (splits > tiles / (2 * kFewWaves)) splits = tiles / (2 * kFewWaves);
+  const long base = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles, cus = device_cus();
+  auto least = [](long a, long b) { return a < b ? a : b; };
+  const long one = least((cus + base - 1) / base, tiles / kFewWaves);
+  const long four = least(4 * cus / base, tiles / (16 * kFewWaves));
+  const long splits = one > four ? one : four;
   p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits);
+  const int per = few_share(static_cast<int>(tiles), p.splits);
+  if (per > 0) p.splits = static_cast<int>((tiles + per - 1) / per);
   return kFew;
 }
 long window_workspace(const WindowArgs& p) {
@@ -756,15 +830,32 @@ extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t s
     window_rows_kernel<<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, stream>>>(p, rows);
   } else if (plan == kPrompt) {
     constexpr int kWaves = 4;
-    p.rows_per_wg = 32 * kWaves / p.hpw;
-    p.n_qblocks = (p.n_q + p.rows_per_wg - 1) / p.rows_per_wg;
-    const long total = static_cast<long>(p.batch) * p.kv_heads * p.n_hgroups * p.n_qblocks;
+    // 32 rows a wave (a K/V fragment read from LDS serves two MFMAs) where that leaves seven workgroups for four CUs,
+    // else 16 (twice the workgroups). 20 query heads on 5 K/V heads, us, 32 / 16 rows: causal 300 tokens 13.1 / 9.4,
+    // 1000: 26.8 / 21.8, two of 1000: 34.9 / 29.5, eight of 300 (400 workgroups of 32 rows): 19.3 / 19.1, 4352 (680):
+    // 138 / 150; all of 4352 to all 211 / 226; 32 on 8 heads, four of 512 (512): 24.5 / 24.8
+    auto groups = [&](int rb) {
+      p.rows_per_wg = 16 * rb * kWaves / p.hpw;
+      p.n_qblocks = (p.n_q + p.rows_per_wg - 1) / p.rows_per_wg;
+      return static_cast<long>(p.batch) * p.kv_heads * p.n_hgroups * p.n_qblocks;
+    };
+    long total = groups(2);
+    const bool few = 4 * total <= 7L * device_cus();
+    if (few) total = groups(1);
     IRIS_REQUIRE(total < (1L << 31), "window_attn: grid too large");
     p.total_wg = static_cast<int>(total);
-    if (p.key_mask)
-      window_attn_kernel<kWaves, 2, 64, true><<<dim3(p.total_wg), 64 * kWaves, 0, stream>>>(p);
-    else
-      window_attn_kernel<kWaves, 2, 64, false><<<dim3(p.total_wg), 64 * kWaves, 0, stream>>>(p);
+    const dim3 grid(p.total_wg);
+    if (few) {
+      if (p.key_mask)
+        window_attn_kernel<1, kWaves, 2, 64, true><<<grid, 64 * kWaves, 0, stream>>>(p);
+      else
+        window_attn_kernel<1, kWaves, 2, 64, false><<<grid, 64 * kWaves, 0, stream>>>(p);
+    } else {
+      if (p.key_mask)
+        window_attn_kernel<2, kWaves, 2, 64, true><<<grid, 64 * kWaves, 0, stream>>>(p);
+      else
+        window_attn_kernel<2, kWaves, 2, 64, false><<<grid, 64 * kWaves, 0, stream>>>(p);
+    }
   } else {
     const long need = window_workspace(p);
     IRIS_REQUIRE(need == 0 || (args->workspace && aligned(args->workspace, 16) && args->workspace_bytes >= need),
