@@ -10,11 +10,13 @@
 // product is already 0.06 radians off. cos and sin of the reduced turn are FP32, the rotation FP32 with
 // one rounding to the output type.
 //
-// Bound by memory: every element is read and written once. A workgroup takes `tok` tokens of one item,
-// computes their (cos, sin) into LDS once for all heads of all tensors, then moves the heads in chunks
-// of 16 bytes (both halves of a pair chunk in one thread, so that a rotation in place is safe);
-// consecutive threads take consecutive chunks of a head, then the next head of the token. Odd widths and
-// strides, and unaligned tensors, go element by element through the same code.
+// Bound by memory: every element is read and written once. A workgroup takes `tok` tokens of one item and
+// tensor, computes their (cos, sin) into LDS once for all heads, and moves the heads in chunks of 16 bytes
+// (both halves of a pair chunk in one thread, so that a rotation in place is safe); consecutive threads take
+// consecutive chunks of a head, then the next head of the token; a thread's loads of four heads go out
+// together, the first before the angles. Odd widths and strides, and unaligned tensors, go element by element
+// through the same code. 4.4 TB/s at 32768 tokens of 32 + 8 BF16 heads (a copy of that size class moves 4.9),
+// 3.1 us for one token of 20 + 5 + 5 heads, 5.5 TB/s at 2 x 4097 FP32 tokens (partly from the cache).
 #include "iris_common.hpp"
 
 namespace iris {
@@ -30,6 +32,9 @@ struct RotaryTensor {
   long os_b, os_h, os_n;  // batch, head, row
   long out_rows;
   int heads, flags;
+  // items of a head: rotated ones (two chunks in the half layout, one in the interleaved), then copied chunks; threads
+  // per head, heads side by side, and the tokens and heads from a thread's head to its next
+  int turning, items, lanes, slots, step_tok, step_h;
 };
 struct RotaryArgs {
   RotaryTensor t[kMaxTensors];
@@ -85,68 +90,87 @@ __device__ __forceinline__ void store_chunk(T* p, const Chunk<T, N>& c) {
 template <typename T, int VEC, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   extern __shared__ f32x2 turns[];  // [tok][pairs] (cos, sin)
+  constexpr int U = 4;              // heads of a thread whose loads are underway together
   const long n0 = static_cast<long>(blockIdx.x) * a.tok;
   const int b = blockIdx.y;
+  const RotaryTensor& t = a.t[blockIdx.z];
+  const int turned = (t.flags & kTurn) ? a.pairs : 0;
+  const bool to_rows = t.flags & kToRows;
   const int ntok = static_cast<int>(a.tokens - n0 < a.tok ? a.tokens - n0 : a.tok);
-  for (int i = threadIdx.x; i < ntok * a.pairs; i += 256) {
-    const int t = i / a.pairs, pair = i - t * a.pairs;
-    const double p = static_cast<double>(index_at(a.positions, a.positions64, b * a.positions_stride + n0 + t));
-    float c, s;
-    turn_of(p, a.freqs[pair], c, s);
-    turns[i] = f32x2{c * a.factor, s * a.factor * a.sign};
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int j = 0; j < a.tensors; ++j) {
-    const RotaryTensor& t = a.t[j];
-    const int turned = (t.flags & kTurn) ? a.pairs : 0;
-    // items of a head: rotated ones (two chunks in the half layout, one in the interleaved), then copied chunks
-    const int turning = INTERLEAVED ? 2 * turned / VEC : turned / VEC;
-    const int items = turning + (a.head_dim - 2 * turned) / VEC;
-    const int lanes = items < 256 ? items : 256;
-    const int slots = 256 / lanes;
-    const int slot = threadIdx.x / lanes, c0 = threadIdx.x - slot * lanes;
-    if (slot >= slots) continue;
-    int tok = slot / t.heads, h = slot - tok * t.heads;
-    while (tok < ntok) {
-      const long n = n0 + tok;
-      const long row = (t.flags & kToRows) ? index_at(a.rows, a.rows64, b * a.rows_stride + n) : n;
-      if (row >= 0 && row < t.out_rows) {
-        const T* x = static_cast<const T*>(t.x) + b * t.xs_b + n * t.xs_n + h * t.xs_h;
-        T* y = static_cast<T*>(t.out) + b * t.os_b + h * t.os_h + row * t.os_n;
-        for (int c = c0; c < items; c += lanes) {
-          if (c >= turning) {
-            const int e = 2 * turned + (c - turning) * VEC;
-            store_chunk<T, VEC>(y + e, load_chunk<T, VEC>(x + e));
-          } else if constexpr (INTERLEAVED) {
-            const int e = c * VEC;
-            const f32x2* cs = turns + tok * a.pairs + e / 2;
-            Chunk<T, VEC> v = load_chunk<T, VEC>(x + e);
+  bool ready = false;  // the first loads go out before the angles are computed
+  auto angles = [&]() {
+    if (ready || turned == 0) return;
+    ready = true;
+    for (int i = threadIdx.x; i < ntok * a.pairs; i += 256) {
+      const int t = i / a.pairs, pair = i - t * a.pairs;
+      const double p = static_cast<double>(index_at(a.positions, a.positions64, b * a.positions_stride + n0 + t));
+      float c, s;
+      turn_of(p, a.freqs[pair], c, s);
+      turns[i] = f32x2{c * a.factor, s * a.factor * a.sign};
+    }
+    __syncthreads();
+  };
+  const int heads = t.heads, turning = t.turning, items = t.items, lanes = t.lanes;
+  const int slot = static_cast<int>(threadIdx.x) / lanes, c0 = threadIdx.x - slot * lanes;
+  const bool on = slot < t.slots;
+  const long x_step = t.step_tok * t.xs_n + t.step_h * t.xs_h, y_step = t.step_h * t.os_h;
+  const long x_wrap = t.xs_n - heads * t.xs_h, y_wrap = heads * t.os_h;
+  const T* const x0 = static_cast<const T*>(t.x) + b * t.xs_b + n0 * t.xs_n;
+  T* const y0 = static_cast<T*>(t.out) + b * t.os_b;
+  for (int c = c0; c - c0 < items; c += lanes) {
+    const bool half = !INTERLEAVED && c < turning;
+    const bool copy = c >= turning;
+    const int e = copy ? 2 * turned + (c - turning) * VEC : c * VEC;
+    const bool here = on && c < items;
+    // (the thread's next head and the offsets of its token and head, kept up by additions)
+    int tok = slot / heads, h = slot - tok * heads;
+    long xo = tok * t.xs_n + h * t.xs_h, yo = h * t.os_h;
+    while (true) {
+      Chunk<T, VEC> u[U], v[U];
+      int toks[U];
+      long ys[U];
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-              const float x0 = to_f32(v.v[2 * i]), x1 = to_f32(v.v[2 * i + 1]);
-              const f32x2 r = cs[i];
-              v.v[2 * i] = from_f32<T>(__builtin_fmaf(x0, r[0], -(x1 * r[1])));
-              v.v[2 * i + 1] = from_f32<T>(__builtin_fmaf(x1, r[0], x0 * r[1]));
-            }
-            store_chunk<T, VEC>(y + e, v);
-          } else {
-            const int e = c * VEC;
-            const f32x2* cs = turns + tok * a.pairs + e;
-            Chunk<T, VEC> u = load_chunk<T, VEC>(x + e), v = load_chunk<T, VEC>(x + e + turned);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              const float x0 = to_f32(u.v[i]), x1 = to_f32(v.v[i]);
-              const f32x2 r = cs[i];
-              u.v[i] = from_f32<T>(__builtin_fmaf(x0, r[0], -(x1 * r[1])));
-              v.v[i] = from_f32<T>(__builtin_fmaf(x1, r[0], x0 * r[1]));
-            }
-            store_chunk<T, VEC>(y + e, u);
-            store_chunk<T, VEC>(y + e + turned, v);
-          }
+      for (int i = 0; i < U; ++i) {
+        toks[i] = here && tok < ntok ? tok : -1;
+        ys[i] = yo;
+        if (toks[i] >= 0) {
+          u[i] = load_chunk<T, VEC>(x0 + xo + e);
+          if (half) v[i] = load_chunk<T, VEC>(x0 + xo + e + turned);
         }
+        tok += t.step_tok, h += t.step_h, xo += x_step, yo += y_step;
+        if (h >= heads) h -= heads, ++tok, xo += x_wrap, yo -= y_wrap;
       }
-      for (h += slots; h >= t.heads; h -= t.heads) ++tok;
+      angles();
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (toks[i] < 0) continue;
+        const long n = n0 + toks[i];
+        const long row = to_rows ? index_at(a.rows, a.rows64, b * a.rows_stride + n) : n;
+        if (row < 0 || row >= t.out_rows) continue;
+        T* const y = y0 + ys[i] + row * t.os_n + e;
+        const f32x2* cs = turns + toks[i] * a.pairs + (INTERLEAVED ? e / 2 : e);
+        if (copy) {
+        } else if constexpr (INTERLEAVED) {
+#pragma unroll
+          for (int q = 0; q < VEC / 2; ++q) {
+            const float f0 = to_f32(u[i].v[2 * q]), f1 = to_f32(u[i].v[2 * q + 1]);
+            const f32x2 r = cs[q];
+            u[i].v[2 * q] = from_f32<T>(__builtin_fmaf(f0, r[0], -(f1 * r[1])));
+            u[i].v[2 * q + 1] = from_f32<T>(__builtin_fmaf(f1, r[0], f0 * r[1]));
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) {
+            const float f0 = to_f32(u[i].v[q]), f1 = to_f32(v[i].v[q]);
+            const f32x2 r = cs[q];
+            u[i].v[q] = from_f32<T>(__builtin_fmaf(f0, r[0], -(f1 * r[1])));
+            v[i].v[q] = from_f32<T>(__builtin_fmaf(f1, r[0], f0 * r[1]));
+          }
+          store_chunk<T, VEC>(y + turned, v[i]);
+        }
+        store_chunk<T, VEC>(y, u[i]);
+      }
+      if (tok >= ntok) break;
     }
   }
 }
@@ -154,7 +178,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 template <typename T>
 void launch_rotary(const RotaryArgs& a, bool vector, int batch, hipStream_t stream) {
   constexpr int kVec = 16 / sizeof(T);
-  const dim3 grid(static_cast<unsigned>((a.tokens + a.tok - 1) / a.tok), batch);
+  const dim3 grid(static_cast<unsigned>((a.tokens + a.tok - 1) / a.tok), batch, a.tensors);
   const size_t lds = static_cast<size_t>(a.tok) * a.pairs * sizeof(f32x2);
   if (a.interleaved) {
     if (vector)
@@ -249,9 +273,9 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
   a.freqs = g.freqs;
   a.factor = static_cast<float>(g.factor);
   a.sign = g.transpose ? -1.0f : 1.0f;
-  // one token per workgroup while that leaves the CUs short of workgroups, up to eight (as many share one
-  // set of launch and index work; more tokens gain nothing)
-  const long per = batch * tokens / (8 * device_cus());
+  // tokens per workgroup, up to eight: four workgroups for every CU (us of 4 x 300 tokens, 20 / 5 heads, at 2, 4, 8 for
+  // every CU: 9.3 / 7.7 / 12.0; 2000 tokens, 32 / 8 heads: 13.3 / 12.2 / 14.2; larger calls alike)
+  const long per = batch * tokens * g.tensors / (4 * device_cus());
   a.tok = static_cast<int>(per < 1 ? 1 : (per > 8 ? 8 : per));
   // chunks of 16 bytes where every chunk of every head is aligned and whole
   const long vec = 16 / size;
@@ -260,6 +284,17 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
     const iris_rotary_tensor& t = g.t[i];
     vector = vector && aligned(t.x, 16) && aligned(t.out, 16);
     for (int d = 0; d < 3; ++d) vector = vector && t.x_strides[d] % vec == 0 && t.out_strides[d] % vec == 0;
+  }
+  for (int i = 0; i < g.tensors; ++i) {
+    RotaryTensor& t = a.t[i];
+    const int turned = (t.flags & kTurn) ? a.pairs : 0;
+    const int chunk = vector ? static_cast<int>(vec) : a.interleaved ? 2 : 1;
+    t.turning = (a.interleaved ? 2 * turned : turned) / chunk;
+    t.items = t.turning + (a.head_dim - 2 * turned) / chunk;
+    t.lanes = t.items < 256 ? t.items : 256;
+    t.slots = 256 / t.lanes;
+    t.step_tok = t.slots / t.heads;
+    t.step_h = t.slots % t.heads;
   }
   if (g.dtype == IRIS_F32)
     launch_rotary<float>(a, vector, static_cast<int>(batch), stream);

@@ -789,14 +789,14 @@ int window_plan(WindowArgs& p) {
     const long reach = (p.causal ? p.window : 2 * p.window - 1) + p.n_q - 1 + 2 * kFewKeys, sinks = p.sinks + kFewKeys;
     keys = reach + sinks < keys ? reach + sinks : keys;
   }
-  // a workgroup for every CU, of one tile a wave at least; where every wave keeps 16 tiles, up to four for every CU.
+  // a workgroup for every CU, of one tile a wave (two rather than a second launch); where every wave keeps 16 tiles, up to four for every CU.
   // us by the number of splits: one token, 20 on 5 heads, 1028 keys 1: 15.2, 4: 11.4, 8: 11.5, 16: 13.1; 4096 keys
   // 4: 20.4, 8: 16.0, 16: 15.6, 32: 17.7; 16384 keys 8: 32.6, 16: 24.6, 32: 22.9; 32 on 8 heads, 65536 keys 16: 82,
   // 32: 66, 64: 76; 16 items of 4096 keys 1: 76, 2: 59, 4: 59, 8: 65; of 65536 keys 1: 1077, 2: 781, 4: 749, 8: 727
   const long tiles = (keys + kFewKeys - 1) / kFewKeys;
   const long base = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles, cus = device_cus();
   auto least = [](long a, long b) { return a < b ? a : b; };
-  const long one = least((cus + base - 1) / base, tiles / kFewWaves);
+  const long one = tiles <= 2 * kFewWaves ? 1 : least((cus + base - 1) / base, (tiles + kFewWaves - 1) / kFewWaves);
   const long four = least(4 * cus / base, tiles / (16 * kFewWaves));
   const long splits = one > four ? one : four;
   p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits);

@@ -148,34 +148,37 @@ def qk_norm_rope(
 _NO_TENSOR = (0,) * 18
 
 
+def _rotary_index(op: str, name: str, t: torch.Tensor, tensors: list) -> tuple[int, int, int]:
+    """Pointer, kind and batch stride of per-token integers for heads whose shape starts ``tensors``."""
+    kind, shape, strides = _INT_KINDS.get(t.dtype, 0), t.shape, t.stride()
+    if (kind == 0 or len(shape) not in (1, 2) or shape[-1] != tensors[2] or (len(shape) == 2 and shape[0] != tensors[1])
+            or (shape[-1] > 1 and strides[-1] != 1)):
+        raise ValueError(f"{op}: {name} must be int32 or int64 [B, N] or [N] with unit stride")
+    return t.data_ptr(), kind, strides[0] if len(shape) == 2 else 0
+
+
 def _rotary(op, xs, outs, turned, to_rows, positions, freqs, rows, layout, factor, transpose) -> None:
     """``iris_rotary`` of ``xs`` into ``outs``: the first ``turned`` rotate, from ``to_rows`` on tokens go to
     ``rows``. (Shapes, strides and overlaps are checked by the library.)"""
     first = xs[0]
-    dtype = _DTYPE_CODES.get(first.dtype)
+    kind = first.dtype
+    dtype = _DTYPE_CODES.get(kind)
     if dtype is None:
-        L.dtype_code(first.dtype)
+        L.dtype_code(kind)
     tensors = []
     for x, out in zip(xs, outs):
-        if x.dtype != first.dtype or out.dtype != first.dtype:
+        if x.dtype != kind or out.dtype != kind:
             raise ValueError(f"{op}: heads and outputs must be of one dtype (got {x.dtype}, {out.dtype})")
-        if x.dim() != 4 or out.dim() != 4:
+        x_shape, out_shape = x.shape, out.shape
+        if len(x_shape) != 4 or len(out_shape) != 4:
             raise ValueError(f"{op}: heads must be [B, N, H, D], outputs [B, H, N, D]")
-        tensors += (x.data_ptr(), *x.shape, *x.stride(), out.data_ptr(), *out.shape, *out.stride())
+        tensors += (x.data_ptr(), *x_shape, *x.stride(), out.data_ptr(), *out_shape, *out.stride())
     if layout not in L.ROTARY_LAYOUTS:
         raise ValueError(f"{op}: layout must be 'half' or 'interleaved', got {layout!r}")
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
         raise ValueError(f"{op}: freqs must be contiguous FP64, one per rotated pair")
-    index = []
-    for name, t in (("positions", positions), ("rows", rows)):
-        if t is None:
-            index += (0, 0, 0)
-            continue
-        kind, shape, wide = _INT_KINDS.get(t.dtype, 0), t.shape, t.dim() == 2
-        if (kind == 0 or t.dim() not in (1, 2) or shape[-1] != first.shape[1] or (wide and shape[0] != first.shape[0])
-                or (shape[-1] > 1 and t.stride(-1) != 1)):
-            raise ValueError(f"{op}: {name} must be int32 or int64 [B, N] or [N] with unit stride")
-        index += (t.data_ptr(), kind, t.stride(0) if wide else 0)
+    index = _rotary_index(op, "positions", positions, tensors)
+    index += (0, 0, 0) if rows is None else index if rows is positions else _rotary_index(op, "rows", rows, tensors)
     n = len(xs)
     args = L.ROTARY_ARGS.pack(n, turned, to_rows, dtype, *tensors, *(_NO_TENSOR * (3 - n)), *index, freqs.data_ptr(),
                               freqs.numel(), L.ROTARY_LAYOUTS[layout], transpose, factor)
