@@ -93,12 +93,19 @@ class HipIris:
     forward over them is recorded once per input shape as a HIP graph (after one eager run,
     whose result that call returns) and replayed by later calls: one launch instead of ~330,
     whatever buffers the caller passes. The result is copied out of the engine's buffer.
+
+    ``core_bits=4`` keeps the two shared adaLN cores, every step's largest read beside the blocks, in 4
+    bits (``kernels.pack_w4``, groups of 64) instead of BF16: a quarter of their memory and traffic, and
+    modulation vectors of the rounded weights.
     """
 
     def __init__(self, cfg: ModelConfig, state_dict: dict[str, torch.Tensor], device: str | torch.device = "cuda",
-                 graphs: bool = True):
+                 graphs: bool = True, core_bits: int = 16):
         cfg.validate()
         check_supported(cfg)
+        if core_bits not in (4, 16):
+            raise ValueError(f"core_bits must be 16 (BF16) or 4, got {core_bits}")
+        self.core_bits = core_bits
         self.cfg = cfg
         self.device = torch.device(device)
         if self.device.type != "cuda":
@@ -114,8 +121,8 @@ class HipIris:
         self.graphs = graphs
 
     @classmethod
-    def from_module(cls, dit, device: str | torch.device = "cuda") -> "HipIris":
-        return cls(dit.cfg, dit.state_dict(), device)
+    def from_module(cls, dit, device: str | torch.device = "cuda", core_bits: int = 16) -> "HipIris":
+        return cls(dit.cfg, dit.state_dict(), device, core_bits=core_bits)
 
     # -- weights ----------------------------------------------------------------------
     def _prepare(self, sd: dict[str, torch.Tensor]) -> None:
@@ -157,8 +164,12 @@ class HipIris:
         self.s_b = f32("s_embedder.proj.bias")
         self.t0_w, self.t0_b = w("t_embedder.mlp.0"), f32("t_embedder.mlp.0.bias")
         self.t2_w, self.t2_b = w("t_embedder.mlp.2"), f32("t_embedder.mlp.2.bias")
-        self.core_img_w, self.core_img_b = w("modulation_cores.adaln_img"), f32("modulation_cores.adaln_img.bias")
-        self.core_txt_w, self.core_txt_b = w("modulation_cores.adaln_txt"), f32("modulation_cores.adaln_txt.bias")
+        def core(name: str):
+            """A shared adaLN core's weight: BF16, or its 4-bit codes and scales."""
+            return w(name) if self.core_bits == 16 else K.pack_w4(sd[f"{name}.weight"].detach().to(dev, torch.float32))[:2]
+
+        self.core_img_w, self.core_img_b = core("modulation_cores.adaln_img"), f32("modulation_cores.adaln_img.bias")
+        self.core_txt_w, self.core_txt_b = core("modulation_cores.adaln_txt"), f32("modulation_cores.adaln_txt.bias")
 
         img_bias, txt_bias = [], []
         self.blocks = []
@@ -431,8 +442,13 @@ class HipIris:
         """Timestep embedding, then both shared adaLN cores with every block's bias folded in."""
         K.timestep_gemv(t, self.t_freqs, self.t0_w, self.t0_b, ws["th"], out_silu=True)
         K.gemv(self.t2_w, ws["th"], self.t2_b, ws["temb"])
-        K.gemv_pair([self.core_img_w, self.core_txt_w], ws["temb"], [self.core_img_b, self.core_txt_b],
-                    [ws["mods_img"], ws["mods_txt"]], [self.img_bias, self.txt_bias], in_silu=True)
+        cores, biases = (self.core_img_w, self.core_txt_w), [self.core_img_b, self.core_txt_b]
+        outs, extra = [ws["mods_img"], ws["mods_txt"]], [self.img_bias, self.txt_bias]
+        if self.core_bits == 16:
+            K.gemv_pair(cores, ws["temb"], biases, outs, extra, in_silu=True)
+        else:
+            (img, img_scales), (txt, txt_scales) = cores
+            K.gemv_w4_pair((img, txt), (img_scales, txt_scales), ws["temb"], biases, outs, extra_biases=extra, in_silu=True)
 
     @torch.no_grad()
     def block_forward(self, index: int, x: torch.Tensor, text: torch.Tensor, t: torch.Tensor,

@@ -112,13 +112,15 @@ def open_weights(checkpoint: str | Path, cfg: ModelConfig, strict: bool = True) 
 
 
 def load_engine(checkpoint: str | Path, device: str | torch.device = "cuda", overrides: dict | None = None,
-                strict: bool = True, graphs: bool = True):
+                strict: bool = True, graphs: bool = True, core_bits: int = 16):
     """``HipIris`` for a released checkpoint directory (src/iris_metal/loading.py:67-77 and
-    pipeline.py:133-142). Tensors are read, converted and moved one at a time."""
+    pipeline.py:133-142). Tensors are read, converted and moved one at a time; ``core_bits``: 16, or 4 for
+    the adaLN cores in 4 bits."""
     from .engine import HipIris
 
     cfg = load_config(checkpoint, overrides)
-    return HipIris(cfg, open_weights(checkpoint, cfg, strict), device=device, graphs=graphs)
+    return HipIris(cfg, open_weights(checkpoint, cfg, strict), device=device, graphs=graphs,
+                   core_bits=core_bits)
 
 
 def load_turbo_sigmas(checkpoint: str | Path) -> tuple[float, ...] | None:
