@@ -487,7 +487,7 @@ int launch_tiles(W4Launch& a, int jobs, hipStream_t stream) {
     if (!fit) continue;
     a.blocks0 = blocks[0];
     const dim3 grid(blocks[0] + blocks[1], (a.batch + a.nb - 1) / a.nb);
-    IRIS_REQUIRE(grid.y < 65536, "gemv_w4: batch too large");
+    IRIS_REQUIRE(grid.y < 65536 && grid.x < (1u << 23), "gemv_w4: too many input or weight rows");
     if (depth == kDepth)
       gemv_w4_kernel<X, PARTS, MT, NT, SPG, kDepth><<<grid, kThreads, lds, stream>>>(a);
     else
@@ -541,8 +541,8 @@ extern "C" int iris_gemv_w4(const iris_gemv_w4_args* args, hipStream_t stream) {
   for (int j = 0; j < g.jobs; ++j) {
     const iris_gemv_w4_job& t = g.job[j];
     IRIS_REQUIRE(t.n > 0 && t.n < (1L << 30), "gemv_w4: bad weight rows");
-    IRIS_REQUIRE(t.n_extra >= 0 && t.n_extra < (1L << 20) && (t.n_extra == 0 || t.extra_bias),
-                 "gemv_w4: extra biases missing");
+    IRIS_REQUIRE(t.n_extra >= 0 && t.n_extra < (1L << 16) && (t.n_extra == 0 || t.extra_bias),
+                 "gemv_w4: extra biases missing, or 65536 and more");
     IRIS_REQUIRE(t.codes && t.scales && (t.out || g.batch == 0), "gemv_w4: null pointer");
     IRIS_REQUIRE(aligned(t.codes, 16), "gemv_w4: codes must be 16-byte aligned");
     const char* out = static_cast<const char*>(t.out);
@@ -560,6 +560,12 @@ extern "C" int iris_gemv_w4(const iris_gemv_w4_args* args, hipStream_t stream) {
                      t.out};
   }
   if (g.batch == 0) return IRIS_OK;
+  if (g.jobs == 2) {
+    const char* first = static_cast<const char*>(g.job[0].out);
+    const char* second = static_cast<const char*>(g.job[1].out);
+    auto bytes = [&](int j) { return (g.job[j].n_extra ? g.job[j].n_extra : 1) * g.batch * g.job[j].n * (g.out_dtype == IRIS_F32 ? 4 : 2); };
+    IRIS_REQUIRE(first + bytes(0) <= second || second + bytes(1) <= first, "gemv_w4: the products' outputs must lie apart");
+  }
   a.x = g.x;
   a.out_dtype = static_cast<int>(g.out_dtype);
   a.batch = static_cast<int>(g.batch);

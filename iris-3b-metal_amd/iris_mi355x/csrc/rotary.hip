@@ -253,12 +253,18 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
     uintptr_t x0, x1, y0, y1;
     extent(t.x, t.x_shape, t.x_strides, 4, size, &x0, &x1);
     extent(t.out, t.out_shape, t.out_strides, 4, size, &y0, &y1);
-    const bool same = t.x == t.out && !to_rows && t.x_strides[0] == t.out_strides[0] &&
-                      t.x_strides[1] == t.out_strides[2] && t.x_strides[2] == t.out_strides[1];
+    const bool same = t.x == t.out && !to_rows && (batch == 1 || t.x_strides[0] == t.out_strides[0]) &&
+                      (tokens == 1 || t.x_strides[1] == t.out_strides[2]) &&
+                      (heads == 1 || t.x_strides[2] == t.out_strides[1]);
     IRIS_REQUIRE(same || x1 <= y0 || y1 <= x0,
                  "rotary: output %d must be its input itself (as [B, H, N, D]) or lie apart from it", i);
   }
   if (batch == 0 || tokens == 0) return IRIS_OK;
+  // (tensors of one projection interleave, so their extents may meet; one tensor given twice is a mistake)
+  for (int i = 0; i < g.tensors; ++i)
+    for (int j = 0; j < g.tensors; ++j)
+      IRIS_REQUIRE(i == j || g.t[i].out_shape[2] == 0 || (g.t[i].out != g.t[j].x && g.t[i].out != g.t[j].out),
+                   "rotary: output %d is another tensor's input or output", i);
   a.tensors = static_cast<int>(g.tensors);
   a.tokens = tokens;
   a.head_dim = static_cast<int>(dim);
@@ -277,6 +283,7 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
   // every CU: 9.3 / 7.7 / 12.0; 2000 tokens, 32 / 8 heads: 13.3 / 12.2 / 14.2; larger calls alike)
   const long per = batch * tokens * g.tensors / (4 * device_cus());
   a.tok = static_cast<int>(per < 1 ? 1 : (per > 8 ? 8 : per));
+  IRIS_REQUIRE((tokens + a.tok - 1) / a.tok < (1L << 24), "rotary: too many tokens");
   // chunks of 16 bytes where every chunk of every head is aligned and whole
   const long vec = 16 / size;
   bool vector = (a.interleaved ? 2 * g.pairs : g.pairs) % vec == 0 && (dim - 2 * g.pairs) % vec == 0;

@@ -720,6 +720,7 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
                "a multiple of K/V heads",
                batch, heads, n_q, g.q_shape[3], g.k_shape[0], kv_heads, n_k, g.k_shape[3]);
   IRIS_REQUIRE(n_q >= 0 && n_k >= 0 && n_q < (1L << 30) && n_k < (1L << 30), "window_attn: need fewer than 2^30 rows");
+  IRIS_REQUIRE(batch * heads * n_q < (1L << 31), "window_attn: need fewer than 2^31 rows of queries and heads");
   IRIS_REQUIRE(g.window >= 0 && g.sinks >= 0, "window_attn: window and sinks must not be negative");
   IRIS_REQUIRE(!g.lengths || g.lengths_kind == 1 || g.lengths_kind == 3, "window_attn: lengths are int32 (1) or int64 (3)");
   IRIS_REQUIRE(g.starts_kind == 0 || g.starts_kind == 4 || ((g.starts_kind == 1 || g.starts_kind == 3) && g.starts),
@@ -732,9 +733,13 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   IRIS_REQUIRE(g.q && g.out && (n_k == 0 || (g.k && g.v)), "window_attn: null pointer");
   IRIS_REQUIRE(aligned(g.q, 16) && aligned(g.k, 16) && aligned(g.v, 16) && aligned(g.out, 8),
                "window_attn: inputs must be 16-byte aligned, the output 8");
-  for (int i = 0; i < 3; ++i)
-    IRIS_REQUIRE(g.q_strides[i] % 8 == 0 && g.k_strides[i] % 8 == 0 && g.v_strides[i] % 8 == 0,
-                 "window_attn: strides must be multiples of 8 elements");
+  // (the stride of an axis of one says nothing)
+  auto stride = [](const long* shape, const long* strides, int i) { return shape[i] > 1 ? strides[i] : (i == 2 ? kHd : 0); };
+  p.qs_b = stride(g.q_shape, g.q_strides, 0), p.qs_h = stride(g.q_shape, g.q_strides, 1), p.qs_n = stride(g.q_shape, g.q_strides, 2);
+  p.ks_b = stride(g.k_shape, g.k_strides, 0), p.ks_h = stride(g.k_shape, g.k_strides, 1), p.ks_n = stride(g.k_shape, g.k_strides, 2);
+  p.vs_b = stride(g.v_shape, g.v_strides, 0), p.vs_h = stride(g.v_shape, g.v_strides, 1), p.vs_n = stride(g.v_shape, g.v_strides, 2);
+  for (long x : {p.qs_b, p.qs_h, p.qs_n, p.ks_b, p.ks_h, p.ks_n, p.vs_b, p.vs_h, p.vs_n})
+    IRIS_REQUIRE(x % 8 == 0 && x >= 0, "window_attn: strides must be multiples of 8 elements, and not negative");
   IRIS_REQUIRE((n_q == 1 || g.out_strides[1] >= heads * kHd) && (batch == 1 || g.out_strides[0] >= heads * kHd) &&
                    g.out_strides[0] % 4 == 0 && g.out_strides[1] % 4 == 0,
                "window_attn: output rows must not overlap, strides must be multiples of 4");
@@ -751,9 +756,6 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   p.k = static_cast<const bf16*>(g.k);
   p.v = static_cast<const bf16*>(g.v);
   p.out = static_cast<bf16*>(g.out);
-  p.qs_b = g.q_strides[0], p.qs_h = g.q_strides[1], p.qs_n = g.q_strides[2];
-  p.ks_b = g.k_strides[0], p.ks_h = g.k_strides[1], p.ks_n = g.k_strides[2];
-  p.vs_b = g.v_strides[0], p.vs_h = g.v_strides[1], p.vs_n = g.v_strides[2];
   p.os_b = g.out_strides[0], p.os_n = g.out_strides[1];
   p.batch = static_cast<int>(batch);
   p.heads = static_cast<int>(heads);
@@ -761,7 +763,7 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   p.n_q = static_cast<int>(n_q);
   p.n_k = static_cast<int>(n_k);
   p.window = g.window < (1L << 60) ? g.window : (1L << 60);
-  p.sinks = g.sinks;
+  p.sinks = g.sinks < (1L << 60) ? g.sinks : (1L << 60);
   p.causal = g.causal != 0;
   p.lengths = g.lengths;
   p.lengths64 = g.lengths_kind == 3;
@@ -824,8 +826,8 @@ extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t s
   const int rc = window_args(args, p);
   if (rc || p.batch == 0) return rc;
   const long rows = static_cast<long>(p.batch) * p.heads * p.n_q;
-  IRIS_REQUIRE(rows < (1L << 31), "window_attn: too many query rows");
   const int plan = window_plan(p);
+  IRIS_REQUIRE(plan == kPrompt || rows < (1L << 26), "window_attn: too many rows of queries and heads");
   if (plan == kRows) {
     window_rows_kernel<<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, stream>>>(p, rows);
   } else if (plan == kPrompt) {
@@ -842,7 +844,7 @@ extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t s
     long total = groups(2);
     const bool few = 4 * total <= 7L * device_cus();
     if (few) total = groups(1);
-    IRIS_REQUIRE(total < (1L << 31), "window_attn: grid too large");
+    IRIS_REQUIRE(total < (1L << 24), "window_attn: too many rows of queries and heads");
     p.total_wg = static_cast<int>(total);
     const dim3 grid(p.total_wg);
     if (few) {
@@ -863,7 +865,7 @@ extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t s
     p.part_o = static_cast<float*>(args->workspace);
     p.part_ml = p.part_o + rows * p.splits * kHd;
     const long total = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles * p.splits;
-    IRIS_REQUIRE(total < (1L << 31), "window_attn: grid too large");
+    IRIS_REQUIRE(total < (1L << 23), "window_attn: too many items and K/V heads");
     p.total_wg = static_cast<int>(total);
     if (p.key_mask)
       window_few_kernel<true><<<dim3(p.total_wg), 64 * kFewWaves, 0, stream>>>(p);

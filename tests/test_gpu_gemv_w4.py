@@ -191,3 +191,9 @@ def test_empty_batch():
     codes, scales, z, x, bias, _ = make(51, 20, 64, 64, 1, False)
     out = torch.empty(0, 20, device=DEV)
     K.gemv_w4(codes, scales, x[:0], bias, out)
+
+
+@pytest.mark.parametrize("extra,batch", [(65535, 2), (9000, 32), (1, 33)])
+def test_many_extra_biases(extra, batch):
+    args = make(49, 17, 64, 32, batch, True, x_dtype=torch.bfloat16, extra=extra)
+    check(run(args, 32, torch.float32), args, 32)

@@ -229,3 +229,14 @@ def test_captured_calls_replay():
         want = K.rotary_store(q, k, v, positions, freqs, caches[2], caches[3])
         assert torch.equal(q_out, want)
         assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+@pytest.mark.parametrize("batch,n,heads", [(1, 3, 2), (2, 1, 3), (2, 3, 1), (1, 1, 1)])
+def test_in_place_with_axes_of_one(batch, n, heads):
+    """The strides of such axes say nothing: a view that differs from the input only there is the input itself."""
+    x = torch.randn(batch, n, heads, 64, generator=torch.Generator(device=DEV).manual_seed(17), device=DEV)
+    positions, (freqs, _) = torch.arange(n, device=DEV) + 9, tables.rotary_frequencies(64, 10000.0, DEV)
+    before = x.clone()
+    strides = [s if size > 1 else 4096 + i for i, (size, s) in enumerate(zip(x.transpose(1, 2).shape, x.transpose(1, 2).stride()))]
+    K.rotary(x, None, positions, freqs, q_out=x.transpose(1, 2).as_strided((batch, heads, n, 64), strides))
+    check(x.transpose(1, 2), before, positions, freqs, "half")

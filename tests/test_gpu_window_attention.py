@@ -253,3 +253,22 @@ def test_streams_and_graphs():
                 graph.replay()
             torch.cuda.current_stream().wait_stream(side)
             assert torch.equal(out, K.window_attention(q, k, v, **opt))
+
+
+@pytest.mark.parametrize("nq", [1, 40])
+def test_strides_of_axes_of_one_say_nothing(nq):
+    """One item, one K/V head, one key: the strides of such axes are never taken, whatever they are."""
+    q, k, v = heads_of(35, 1, nq, 70, 2, 1)
+    want = K.window_attention(q, k, v, window=9)
+    odd = [t.as_strided(t.shape, (12345, 777 if t.shape[1] == 1 else t.stride(1), *t.stride()[2:])) for t in (q, k, v)]
+    assert torch.equal(K.window_attention(*odd, window=9), want)
+    one = [t[:, :, :1].as_strided((1, 1, 1, 128), (3, 5, s, 1)) for t, s in ((k, 7), (v, 1 << 30))]
+    got = K.window_attention(q, *one, causal=False)
+    assert torch.equal(got.unflatten(-1, (2, 128)), v[:, :, :1].expand(1, nq, 2, 128))
+
+
+def test_key_mask_shared_by_the_items():
+    q, k, v = heads_of(36, 3, 100, 100, 4, 1)
+    mask = torch.rand(1, 100, generator=torch.Generator().manual_seed(5)).to(DEV) < 0.6
+    check(q, k, v, key_mask=mask.expand(3, -1), window=40, sinks=2)
+    check(q[:, :, -1:], k, v, key_mask=mask.expand(3, -1))

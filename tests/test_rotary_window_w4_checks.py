@@ -1,5 +1,7 @@
 """Refusals of the rotary, windowed attention and 4-bit entry points: wrappers and C ABI, on the CPU."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -222,3 +224,67 @@ def test_c_entry_points_refuse():
     for name in names:
         with pytest.raises(ValueError, match="null"):
             _lib.call(name, None, None)
+
+
+def test_rotary_refuses_one_tensor_given_twice(unplaced):
+    """The output of one tensor as the input or output of another, which would race."""
+    q, k = torch.zeros(2, 5, 2, 64), torch.zeros(2, 5, 2, 64)
+    args = (torch.zeros(5, dtype=torch.int64), torch.zeros(32, dtype=torch.float64))
+    out = torch.zeros(2, 2, 5, 64)
+    with pytest.raises(ValueError, match="another tensor"):
+        K.rotary(q, k, *args, q_out=out, k_out=out)
+    with pytest.raises(ValueError, match="another tensor"):
+        K.rotary(q, k, *args, q_out=k.transpose(1, 2))
+    cache = torch.zeros(2, 2, 9, 64)
+    with pytest.raises(ValueError, match="another tensor"):
+        K.rotary_store(q, k, torch.zeros_like(k), *args, cache, cache)
+
+
+def test_gemv_w4_pair_refuses_outputs_that_meet(unplaced):
+    codes, scales = [torch.zeros(6, 64, dtype=torch.uint8)] * 2, [torch.zeros(6, 2)] * 2
+    store = torch.zeros(40)
+    with pytest.raises(ValueError, match="lie apart"):
+        K.gemv_w4_pair(codes, scales, torch.zeros(3, 128), (None, None), (store[:18].view(3, 6), store[17:35].view(3, 6)))
+
+
+def test_size_limits():
+    """Sizes whose products leave 32 bits, and strides that the kernels' offsets cannot express, are turned away
+    before any launch (pointers are never followed)."""
+    at, rows = 1 << 20, 1 << 29
+    shape = dict(q=at, k=at, v=at, out=1 << 50)
+
+    def attn(name, heads, n_q, n_k, k_stride=128, sinks=0, window=0, batch=1):
+        q = (batch, heads, n_q, 128, heads * n_q * 128, n_q * 128, 128, 1)
+        k = (batch, 1, n_k, 128, 0, 0, k_stride, 1)
+        out = (batch, n_q, heads * 128, n_q * heads * 128, heads * 128, 1)
+        args = _lib.WINDOW_ATTN_ARGS.pack(*shape.values(), *q, *k, *k, *out, window, sinks, 1, 0, 0, 0, 0, 0, 0, 0, 0.1, 0, 0)
+        if name == "iris_window_attn":
+            _lib.call(name, args, None)
+            return None
+        need = ctypes.c_long(-1)
+        _lib.call(name, args, ctypes.byref(need))
+        return need.value
+
+    for name in ("iris_window_attn", "iris_window_attn_workspace"):
+        with pytest.raises(ValueError, match="2\\^31"):  # (2^32 rows, 0 in 32 bits)
+            attn(name, 8, rows, 64)
+        with pytest.raises(ValueError, match="not negative"):
+            attn(name, 4, 1, 4096, k_stride=-128)
+    # the largest sinks count as all keys: the same splits, hence workspace, as without a window
+    plain = attn("iris_window_attn_workspace", 4, 1, 65536)
+    assert plain > 0 and attn("iris_window_attn_workspace", 4, 1, 65536, sinks=2**63 - 1, window=5) == plain
+    with pytest.raises(ValueError, match="workspace"):
+        attn("iris_window_attn", 4, 1, 65536)
+    with pytest.raises(ValueError, match="too many"):  # a grid of 2^32 threads and more
+        attn("iris_window_attn", 16384, 1, 8, batch=16384)
+    job = dict(codes=at, scales=at, zeros=0, bias=0, extra_bias=0, out=1 << 50, n=(1 << 30) - 1, n_extra=0)
+    with pytest.raises(ValueError, match="too many"):
+        _lib.call("iris_gemv_w4", _lib.GEMV_W4_ARGS.pack(2, 1, 32, 32, 0, 0, 1, 0, 0, at, *job.values(),
+                                                         *{**job, "out": 1 << 51}.values()), None)
+    with pytest.raises(ValueError, match="65536"):
+        job.update(n=16, n_extra=65536, extra_bias=at)
+        _lib.call("iris_gemv_w4", _lib.GEMV_W4_ARGS.pack(1, 1, 32, 32, 0, 0, 1, 0, 0, at, *job.values(), *(0,) * 8), None)
+    tokens = 1 << 28
+    head = (at, 1, tokens, 1, 64, 64 * tokens, 64, 64, 1, 1 << 50, 1, 1, tokens, 64, 64 * tokens, 64 * tokens, 64, 1)
+    with pytest.raises(ValueError, match="too many"):
+        _lib.call("iris_rotary", _lib.ROTARY_ARGS.pack(1, 1, 3, 0, *head, *(0,) * 36, at, 1, 0, 0, 0, 0, at, 32, 0, 0, 1.0), None)
