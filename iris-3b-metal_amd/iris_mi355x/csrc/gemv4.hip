@@ -20,6 +20,9 @@
 // - The FP32 sums of a group of at least 32 are scaled and added to the row's FP32 sums.
 // A workgroup's eight waves are dealt over weight tiles and over k (their sums joined in LDS): many tiles where
 // the weight has rows enough for all CUs, because every workgroup lays out all inputs anew, few where it has not.
+// One row, 131072 x 4096: 60 us, 4.6 TB/s (a large copy moves 4.9). Small calls are bound by their chain of latencies:
+// inputs and scales to LDS, products, the join of the waves, the store: 6.3 us for 2560 x 2560 of which a launch that
+// does nothing takes about 3; 11.9 us for two FP32 rows, 15360 x 2560, 24 outputs; 14.8 us for 24 rows, 13696 x 2560.
 #include "iris_common.hpp"
 
 namespace iris {
@@ -29,9 +32,8 @@ constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kMaxRows = 48;  // A rows of a workgroup
 constexpr int kAhead = 8;     // extra biases of a thread that are loaded at the start
 constexpr int kScaleItems = 8;  // scales of a thread and stage
-// LDS of a workgroup (inputs and scales of one stage of k, or of two): two workgroups per CU, or one where no CU
-// gets a second
-constexpr int kLdsTwo = 78 << 10, kLdsOne = 156 << 10;
+// LDS of a workgroup (inputs and scales of all k, or of two stages of k) where a CU holds two of them, and at most
+constexpr size_t kLdsTwo = 78 << 10, kLdsOne = 156 << 10;
 
 struct W4Job {
   const unsigned char* codes;
@@ -93,9 +95,11 @@ constexpr int input_items() { return sizeof(X) == 2 ? 8 : 4; }
 
 // X: the inputs' type; PARTS: A rows per input row, 1, or 3 for FP32 and activated inputs; MT tiles of 16 A rows, NT
 // of 16 weight rows per wave; SPG 32-wide k-steps per scale; DEPTH code loads (NT of 16 rows x 128 k each) underway
-// per wave, which divides a stage's chunks of a wave where there are several stages.
-template <typename X, int PARTS, int MT, int NT, int SPG, int DEPTH>
-__global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
+// per wave, which divides a stage's chunks of a wave where there are several stages (STAGED). Without stages nothing
+// of a next one waits in registers, and two workgroups share a CU (one row, 65536 x 4096: 39 us staged, 32 whole).
+template <typename X, int PARTS, int MT, int NT, int SPG, int DEPTH, bool STAGED>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(MT == 1 && !STAGED ? 4 : 2))) void
+gemv_w4_kernel(W4Launch a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ int odd;
   constexpr int XI = input_items<X>();
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
     g0 = group_of(a, k0 >> 5);
     gn = min(group_of(a, (min(k0 + kc, k) - 1) >> 5) - g0 + 1, gs);
   };
-  auto load_scales = [&](int k0) {
+  auto load_scales = [&](int k0, int from) {
     int g0, gn;
     stage_group(k0, g0, gn);
     const Divisor by_gn(gn);
@@ -144,34 +148,34 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
 #pragma unroll
     for (int u = 0; u < kScaleItems; ++u) {
       int r, q;
-      by_gn(min(tid + u * kThreads, n_wg * gn - 1), r, q);
+      by_gn(min(from + tid + u * kThreads, n_wg * gn - 1), r, q);
       at[u] = min(r, most_r) * a.groups + g0 + q;
     }
     if (a.scales_f32) {
 #pragma unroll
       for (int u = 0; u < kScaleItems; ++u)
-        if (w * 64 + u * kThreads < n_wg * gn) scale[u] = *reinterpret_cast<const unsigned*>(scale_at + 4L * at[u]);
+        if (from + w * 64 + u * kThreads < n_wg * gn) scale[u] = *reinterpret_cast<const unsigned*>(scale_at + 4L * at[u]);
     } else {
 #pragma unroll
       for (int u = 0; u < kScaleItems; ++u)
-        if (w * 64 + u * kThreads < n_wg * gn) scale[u] = *reinterpret_cast<const unsigned short*>(scale_at + 2L * at[u]);
+        if (from + w * 64 + u * kThreads < n_wg * gn) scale[u] = *reinterpret_cast<const unsigned short*>(scale_at + 2L * at[u]);
     }
     if (job.zeros) {
 #pragma unroll
       for (int u = 0; u < kScaleItems; ++u)
-        if (w * 64 + u * kThreads < n_wg * gn) zero[u] = zero_at[at[u]];
+        if (from + w * 64 + u * kThreads < n_wg * gn) zero[u] = zero_at[at[u]];
     }
   };
-  auto lay_scales = [&](int k0, char* stage) {
+  auto lay_scales = [&](int k0, char* stage, int from) {
     uint2* const sc = reinterpret_cast<uint2*>(stage + a.nb * PARTS * xs);
     int g0, gn;
     stage_group(k0, g0, gn);
     const Divisor by_gn(gn);
 #pragma unroll
     for (int u = 0; u < kScaleItems; ++u)
-      if (w * 64 + u * kThreads < n_wg * gn) {  // (whole waves; past the last item, it again)
+      if (from + w * 64 + u * kThreads < n_wg * gn) {  // (whole waves; past the last item, it again)
         int r, q;
-        by_gn(min(tid + u * kThreads, n_wg * gn - 1), r, q);
+        by_gn(min(from + tid + u * kThreads, n_wg * gn - 1), r, q);
         // (exact: an integer below 2^8)
         const unsigned h = bits_of(-16.0f - (job.zeros ? static_cast<float>(zero[u]) : 8.0f)) >> 16;
         sc[r * gs + q] = uint2{a.scales_f32 ? scale[u] : scale[u] << 16, h | h << 16};
@@ -182,23 +186,23 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
   const X* const x_at = static_cast<const X*>(a.x) + static_cast<long>(b0) * k;
   constexpr int XW = sizeof(X) / 2;  // 16-byte words of an item
   uint4 xr[XI][XW];
-  auto load_inputs = [&](int k0) {
+  auto load_inputs = [&](int k0, int from) {
 #pragma unroll
     for (int u = 0; u < XI; ++u)
-      if (w * 64 + u * kThreads < items) {
+      if (from + w * 64 + u * kThreads < items) {
         int r, e;
-        by_eights(min(tid + u * kThreads, items - 1), r, e);
+        by_eights(min(from + tid + u * kThreads, items - 1), r, e);
         const uint4* x = reinterpret_cast<const uint4*>(x_at + r * k + min(k0 + 8 * e, k - 8));
 #pragma unroll
         for (int i = 0; i < XW; ++i) xr[u][i] = x[i];
       }
   };
-  auto lay_inputs = [&](int k0, char* stage) {
+  auto lay_inputs = [&](int k0, char* stage, int from) {
 #pragma unroll
     for (int u = 0; u < XI; ++u)
-      if (w * 64 + u * kThreads < items) {
+      if (from + w * 64 + u * kThreads < items) {
         int r, e;
-        by_eights(min(tid + u * kThreads, items - 1), r, e);
+        by_eights(min(from + tid + u * kThreads, items - 1), r, e);
         e *= 8;
         const unsigned keep = k0 + e < k ? ~0u : 0u;
         uint4 v = xr[u][0];
@@ -241,8 +245,8 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
       }
   };
 
-  load_scales(0);
-  load_inputs(0);
+  load_scales(0, 0);
+  load_inputs(0, 0);
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) load(d, wave_k + d * wk);
   // the output's row of this thread (n_wg divides the threads) and its first biases, underway from the start too
@@ -260,8 +264,18 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
       ahead[u] = job.extra[static_cast<long>(j) * n + out_at];
     }
   }
-  lay_scales(0, lds);
-  lay_inputs(0, lds);
+  lay_scales(0, lds, 0);
+  lay_inputs(0, lds, 0);
+  if constexpr (!STAGED) {  // (what the first registers did not hold)
+    for (int from = kScaleItems * kThreads; from < n_wg * gs; from += kScaleItems * kThreads) {
+      load_scales(0, from);
+      lay_scales(0, lds, from);
+    }
+    for (int from = XI * kThreads; from < items; from += XI * kThreads) {
+      load_inputs(0, from);
+      lay_inputs(0, lds, from);
+    }
+  }
   lds_barrier();
 
   f32x4 acc[MT][NT];
@@ -279,10 +293,10 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
   const int mine = (chunks - wave_k + wk - 1) / wk;  // of this wave in all
   char* stage = lds;
   for (int k0 = 0, i0 = 0; k0 < k; k0 += kc, i0 += per_stage) {
-    const bool more = k0 + kc < k;
+    const bool more = STAGED && k0 + kc < k;
     if (more) {
-      load_scales(k0 + kc);
-      load_inputs(k0 + kc);
+      load_scales(k0 + kc, 0);
+      load_inputs(k0 + kc, 0);
     }
     const uint2* const sc = reinterpret_cast<const uint2*>(stage + a.nb * PARTS * xs);
     int g0, gn;
@@ -359,8 +373,8 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
       if (i + d < here) chunk(d, wave_k + (i0 + i + d) * wk, false);
     if (more) {
       stage = stage == lds ? lds + stage_bytes : lds;  // (its last readers are a barrier behind)
-      lay_scales(k0 + kc, stage);
-      lay_inputs(k0 + kc, stage);
+      lay_scales(k0 + kc, stage, 0);
+      lay_inputs(k0 + kc, stage, 0);
       lds_barrier();
     }
   }
@@ -443,58 +457,66 @@ __global__ __launch_bounds__(kThreads) void gemv_w4_kernel(W4Launch a) {
 // that depth does not fit.
 template <typename X, int PARTS, int MT, int NT>
 size_t plan_job(const W4Launch& a, W4Job& job, int& blocks, int depth) {
-  const int cus = device_cus();
+  auto bytes = [&](int wn, int kc) {  // of a stage
+    return static_cast<size_t>(a.nb) * PARTS * x_stride(kc) + static_cast<size_t>(wn) * NT * 16 * stage_groups(kc, a.group) * 8;
+  };
+  auto whole = [&](int wn) { return (a.k + 128 * (kWaves / wn) - 1) / (128 * (kWaves / wn)) * (128 * (kWaves / wn)); };
   // as many weight rows per workgroup as leave four of five CUs a workgroup (by the product's own rows, so that a
-  // result does not depend on the other product of a launch)
+  // result does not depend on the other product of a launch; twice the workgroups of half the rows, us: 2 FP32 rows,
+  // 15360 x 2560 12.5 instead of 11.9, 15360 x 5120 26.8 / 15.7; 24 BF16 rows, 13696 x 2560 24.6 / 14.8), and half of
+  // that where a CU then holds two (one row, 32768 x 8192: 33.8 instead of 39.9; where all of k only then is one stage
+  // it loses: 4 FP32 rows, 32768 x 4096 27.8 / 23.8)
+  constexpr int kLeast = MT > 2 ? 2 : 1;
   job.wn = kWaves;
-  while (job.wn > (MT > 2 ? 2 : 1) && 5L * job.n < 4L * job.wn * NT * 16 * cus) job.wn /= 2;
+  while (job.wn > kLeast && 5L * job.n < 4L * job.wn * NT * 16 * device_cus()) job.wn /= 2;
+  if (job.wn > kLeast && bytes(job.wn, whole(job.wn)) > kLdsTwo && bytes(job.wn / 2, whole(job.wn / 2)) <= kLdsTwo) job.wn /= 2;
   const int n_wg = job.wn * NT * 16, wk = kWaves / job.wn;
   blocks = (job.n + n_wg - 1) / n_wg;
-  int most = blocks <= cus ? kLdsOne : kLdsTwo;
-  auto bytes = [&](int kc) { return a.nb * PARTS * x_stride(kc) + n_wg * stage_groups(kc, a.group) * 8; };
-  auto fits = [&](int kc, int stages) {
-    return a.nb * (kc / 8) <= input_items<X>() * kThreads && n_wg * stage_groups(kc, a.group) <= kScaleItems * kThreads &&
-           stages * bytes(kc) <= most;
-  };
-  const int whole = (a.k + 128 * wk - 1) / (128 * wk) * (128 * wk);
   const size_t sums = static_cast<size_t>(wk) * n_wg * (MT * 16 + 1) * 4;
-  size_t lds;
-  if (fits(whole, 1)) {
-    job.kc = whole;
-    lds = bytes(whole);
+  size_t lds = bytes(job.wn, whole(job.wn));
+  if (lds <= kLdsOne) {
+    job.kc = whole(job.wn);
   } else {
+    auto fits = [&](int kc) {  // (a stage's inputs and scales are in registers while the stage before is computed)
+      return a.nb * (kc / 8) <= input_items<X>() * kThreads && n_wg * stage_groups(kc, a.group) <= kScaleItems * kThreads &&
+             2 * bytes(job.wn, kc) <= kLdsOne;
+    };
     const int unit = 128 * wk * depth;
-    if (!fits(unit, 2)) most = kLdsOne;
-    if (!fits(unit, 2)) return 0;
-    for (job.kc = unit; fits(job.kc + unit, 2);) job.kc += unit;
-    lds = 2 * static_cast<size_t>(bytes(job.kc));
+    if (!fits(unit)) return 0;
+    for (job.kc = unit; fits(job.kc + unit);) job.kc += unit;
+    lds = 2 * bytes(job.wn, job.kc);
   }
   return lds > sums ? lds : sums;
 }
 
+// Launches with DEPTH code loads underway, if that fits; 1 where it does not.
+template <typename X, int PARTS, int MT, int NT, int SPG, int DEPTH>
+int launch_depth(W4Launch& a, int jobs, bool staged, hipStream_t stream) {
+  size_t lds = 0;
+  int blocks[2] = {0, 0};
+  for (int j = 0; j < jobs; ++j) {
+    const size_t need = plan_job<X, PARTS, MT, NT>(a, a.job[j], blocks[j], DEPTH);
+    if (need == 0 || (!staged && a.job[j].kc < a.k)) return 1;
+    lds = need > lds ? need : lds;
+  }
+  a.blocks0 = blocks[0];
+  const dim3 grid(blocks[0] + blocks[1], (a.batch + a.nb - 1) / a.nb);
+  IRIS_REQUIRE(grid.y < 65536 && grid.x < (1u << 23), "gemv_w4: too many input or weight rows");
+  if (staged)
+    gemv_w4_kernel<X, PARTS, MT, NT, SPG, DEPTH, true><<<grid, kThreads, lds, stream>>>(a);
+  else if constexpr (DEPTH > 1)
+    gemv_w4_kernel<X, PARTS, MT, NT, SPG, DEPTH, false><<<grid, kThreads, lds, stream>>>(a);
+  return check_launch("gemv_w4");
+}
+
 template <typename X, int PARTS, int MT, int NT, int SPG>
 int launch_tiles(W4Launch& a, int jobs, hipStream_t stream) {
-  constexpr int kDepth = MT == 1 ? 4 : 2;  // (more registers spill)
-  for (int depth = kDepth; depth >= 1; depth -= kDepth - 1) {
-    size_t lds = 0;
-    int blocks[2] = {0, 0};
-    bool fit = true;
-    for (int j = 0; j < jobs; ++j) {
-      const size_t need = plan_job<X, PARTS, MT, NT>(a, a.job[j], blocks[j], depth);
-      fit = fit && need > 0;
-      lds = need > lds ? need : lds;
-    }
-    if (!fit) continue;
-    a.blocks0 = blocks[0];
-    const dim3 grid(blocks[0] + blocks[1], (a.batch + a.nb - 1) / a.nb);
-    IRIS_REQUIRE(grid.y < 65536 && grid.x < (1u << 23), "gemv_w4: too many input or weight rows");
-    if (depth == kDepth)
-      gemv_w4_kernel<X, PARTS, MT, NT, SPG, kDepth><<<grid, kThreads, lds, stream>>>(a);
-    else
-      gemv_w4_kernel<X, PARTS, MT, NT, SPG, 1><<<grid, kThreads, lds, stream>>>(a);
-    return check_launch("gemv_w4");
-  }
-  return fail(IRIS_E_UNSUPPORTED, "gemv_w4: no stage of k fits");  // (one of 128 k per wave always does)
+  // (more registers spill; with two workgroups on a CU two loads a wave do as well as four: 15360 x 5120 15.7 / 16.3 us)
+  constexpr int kDepth = MT == 1 ? 4 : 2;
+  int rc = launch_depth<X, PARTS, MT, NT, SPG, 2>(a, jobs, false, stream);
+  if (rc == 1) rc = launch_depth<X, PARTS, MT, NT, SPG, kDepth>(a, jobs, true, stream);
+  if (rc == 1) rc = launch_depth<X, PARTS, MT, NT, SPG, 1>(a, jobs, true, stream);
+  return rc == 1 ? fail(IRIS_E_UNSUPPORTED, "gemv_w4: no stage of k fits") : rc;  // (one of 128 k per wave always does)
 }
 
 template <typename X, int PARTS, int SPG>
