@@ -14,11 +14,14 @@
 // 16 lanes). Only tiles that hold a visible key of some query of the workgroup are visited.
 //
 // window_attn_kernel (prompts): bound by the MFMAs and the softmax beside them. A workgroup's waves share a
-// ring of K/V tiles; a wave is one query head's 32 rows, the heads of a K/V head side by side.
+// ring of K/V tiles; a wave is one query head's 16 or 32 rows, the heads of a K/V head side by side. 8192 tokens, 32 on 8
+// heads, window 4096: 391 us, 1054 TFLOP/s of visible pairs; 4352 tokens, 20 on 5, two-sided window 640 and 256 first
+// keys: 88 us, 705 TFLOP/s (680 workgroups in 512 places); small prompts are a chain of 5 us and 0.8 us per tile.
 // window_few_kernel (few queries): bound by the keys' and values' way from memory. The rows of a tile are the
 // (query, head) pairs of one K/V head; every wave streams key tiles of its own through its own LDS, without
-// barriers, and the waves' and workgroups' parts are joined at the end (window_join_kernel for the latter).
-// window_rows_kernel: row strides too large for the 32-bit offsets of the others.
+// barriers, and the waves' and workgroups' parts are joined at the end (window_join_kernel for the latter). 16 queries
+// of 32 on 8 heads over 65536 keys at most: 599 us, 5.5 TB/s; one query over 1028 keys: 11 us in two launches.
+// window_rows_kernel: row strides of 2^24 elements and more, too large for the 32-bit offsets of the others.
 #include "iris_common.hpp"
 
 #include <type_traits>
@@ -782,23 +785,29 @@ int window_plan(WindowArgs& p) {
   if (p.ks_n >= (1L << 24) || p.vs_n >= (1L << 24)) return kRows;  // (32 rows of a tile by 32-bit offsets)
   p.hpw = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
   p.n_hgroups = group / p.hpw;
-  if (rows > 64)  // (all rows by 32-bit offsets)
-    return (p.n_k + 64) * (p.ks_n > p.vs_n ? p.ks_n : p.vs_n) * 2 < (1L << 31) ? kPrompt : kRows;
   p.row_tiles = (rows + 15) / 16;
-  // keys that the queries can see at most, in tiles
+  const long base = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles, cus = device_cus();
+  // Few: no more 16-row tiles than CUs, so that the prompts' form, a wave for 16 rows of a head with all of its keys,
+  // would leave most waves of the card without work. us, few / prompts: 20 on 5 heads, 16 queries of 32768 keys 68 / 605, 32:
+  // 101 / 575, 64 of 4096 keys: 26 / 61, 128 of 1000 (160 tiles): 16 / 18, of 16384: 135 / 224; 8 on 1 head, 400 of 1000
+  // (200): 15.5 / 18; beyond: 32 items of 16 queries, 1024 keys (640) 49 / 27; 64 items of one query, 2048 keys (320)
+  // 81 / 68. (The prompts' form reaches all rows by 32-bit offsets; this one those of a tile.)
+  if (base > cus && (p.n_k + 64) * (p.ks_n > p.vs_n ? p.ks_n : p.vs_n) * 2 < (1L << 31)) return kPrompt;
+  // keys that a tile's queries can see at most, in tiles
   long keys = p.n_k;
   if (p.window) {
-    const long reach = (p.causal ? p.window : 2 * p.window - 1) + p.n_q - 1 + 2 * kFewKeys, sinks = p.sinks + kFewKeys;
+    const long queries = p.n_q < 15 / group + 2 ? p.n_q : 15 / group + 2;
+    const long reach = (p.causal ? p.window : 2 * p.window - 1) + queries - 1 + 2 * kFewKeys, sinks = p.sinks + kFewKeys;
     keys = reach + sinks < keys ? reach + sinks : keys;
   }
-  // a workgroup for every CU, of one tile a wave (two rather than a second launch); where every wave keeps 16 tiles, up to four for every CU.
+  // as many workgroups as CUs, of one tile a wave (two rather than a second launch; one more than CUs is a second
+  // round: 128 queries of 1000 keys 23 instead of 16 us); where every wave keeps 16 tiles, up to four for every CU.
   // us by the number of splits: one token, 20 on 5 heads, 1028 keys 1: 15.2, 4: 11.4, 8: 11.5, 16: 13.1; 4096 keys
   // 4: 20.4, 8: 16.0, 16: 15.6, 32: 17.7; 16384 keys 8: 32.6, 16: 24.6, 32: 22.9; 32 on 8 heads, 65536 keys 16: 82,
   // 32: 66, 64: 76; 16 items of 4096 keys 1: 76, 2: 59, 4: 59, 8: 65; of 65536 keys 1: 1077, 2: 781, 4: 749, 8: 727
   const long tiles = (keys + kFewKeys - 1) / kFewKeys;
-  const long base = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles, cus = device_cus();
   auto least = [](long a, long b) { return a < b ? a : b; };
-  const long one = tiles <= 2 * kFewWaves ? 1 : least((cus + base - 1) / base, (tiles + kFewWaves - 1) / kFewWaves);
+  const long one = tiles <= 2 * kFewWaves ? 1 : least(cus / base, (tiles + kFewWaves - 1) / kFewWaves);
   const long four = least(4 * cus / base, tiles / (16 * kFewWaves));
   const long splits = one > four ? one : four;
   p.splits = static_cast<int>(splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits);

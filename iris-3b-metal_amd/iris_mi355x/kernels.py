@@ -827,13 +827,11 @@ def window_attention(
             lengths_kind, starts_at, starts_kind, start, mask_at, mask_stride,
             HEAD_DIM ** -0.5 if scale is None else scale]
     stream = _on_current_device("window_attention", q, k, v, out, lengths, starts, key_mask)
-    workspace = None
-    if heads * n_q <= 64 * k_shape[1]:  # few queries: their keys may be split
-        need = ctypes.c_long()
-        L.call("iris_window_attn_workspace", L.WINDOW_ATTN_ARGS.pack(*args, 0, 0), ctypes.byref(need))
-        if need.value:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-            args += (workspace.data_ptr(), need.value)
+    workspace, need = None, ctypes.c_long()  # (few queries: their keys may be split)
+    L.call("iris_window_attn_workspace", L.WINDOW_ATTN_ARGS.pack(*args, 0, 0), ctypes.byref(need))
+    if need.value:
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        args += (workspace.data_ptr(), need.value)
     L.call("iris_window_attn", L.WINDOW_ATTN_ARGS.pack(*args, *((0, 0) if workspace is None else ())), stream)
     return out
 

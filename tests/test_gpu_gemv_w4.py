@@ -197,3 +197,34 @@ def test_empty_batch():
 def test_many_extra_biases(extra, batch):
     args = make(49, 17, 64, 32, batch, True, x_dtype=torch.bfloat16, extra=extra)
     check(run(args, 32, torch.float32), args, 32)
+
+
+@pytest.mark.parametrize("batch,k,x_dtype,in_silu", [
+    (1, 81920, torch.bfloat16, False), (16, 9984, torch.bfloat16, False), (27, 6848, torch.bfloat16, False),
+    (32, 12288, torch.bfloat16, False), (1, 30016, torch.float32, False), (5, 8192, torch.float32, True),
+    (9, 6880, torch.float32, False), (16, 4128, torch.float32, True), (5, 9984, torch.bfloat16, True),
+    (16, 9984, torch.bfloat16, True)])
+@pytest.mark.parametrize("group", [32, 128, 4096])
+@pytest.mark.parametrize("n", [40, 2100])
+def test_k_in_stages(batch, k, x_dtype, in_silu, group, n):
+    """Inputs that fill more than a workgroup's LDS, few and many waves side by side."""
+    args = make(50, n, k, group, batch, True, x_dtype=x_dtype)
+    check(run(args, group, torch.float32, in_silu=in_silu), args, group, in_silu=in_silu)
+
+
+@pytest.mark.parametrize("batch,k,x_dtype", [(16, 9984, torch.bfloat16), (28, 4992, torch.bfloat16), (4, 8192, torch.float32),
+                                             (14, 2592, torch.float32)])
+def test_k_in_stages_of_many_rows(batch, k, x_dtype):
+    args = make(51, 30001, k, 64, batch, False, x_dtype=x_dtype)
+    check(run(args, 64, torch.float32), args, 64)
+
+
+def test_pair_of_which_one_takes_stages():
+    jobs = [make(52 + i, n, 4096, 64, 4, False) for i, n in enumerate((30000, 40))]
+    x = jobs[0][3]
+    outs = [[torch.full((4, a[0].shape[0]), 7.0, device=DEV) for a in jobs] for _ in range(2)]
+    K.gemv_w4_pair([a[0] for a in jobs], [a[1] for a in jobs], x, [a[4] for a in jobs], outs[0], 64)
+    for a, out, got in zip(jobs, outs[1], outs[0]):
+        K.gemv_w4(a[0], a[1], x, a[4], out, 64)
+        assert torch.equal(got, out)
+        check(got, (*a[:3], x, *a[4:]), 64)

@@ -272,3 +272,73 @@ def test_key_mask_shared_by_the_items():
     mask = torch.rand(1, 100, generator=torch.Generator().manual_seed(5)).to(DEV) < 0.6
     check(q, k, v, key_mask=mask.expand(3, -1), window=40, sinks=2)
     check(q[:, :, -1:], k, v, key_mask=mask.expand(3, -1))
+
+
+# Calls of more 16-row tiles than the card has CUs (and of K/V that 32-bit offsets do not span)
+@pytest.mark.parametrize("n", [17, 33, 64, 65, 130, 200])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (7, 1), (64, 4), (100, 70), (1000, 3)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_prompts(n, window, sinks, causal):
+    q, k, v = heads_of(37, 20, n, n, 8, 8, gain=2.0)
+    check(q, k, v, window=window, sinks=sinks, causal=causal)
+
+
+@pytest.mark.parametrize("heads,kv,batch", [(20, 5, 60), (5, 5, 70), (6, 2, 150), (6, 1, 300), (32, 2, 80)])
+@pytest.mark.parametrize("nq,nk", [(1, 300), (3, 77), (16, 129)])
+def test_few_queries_of_many_items(heads, kv, batch, nq, nk):
+    q, k, v = heads_of(38, batch, nq, nk, heads, kv)
+    g = torch.Generator(device=DEV).manual_seed(39)
+    lengths = torch.randint(0, nk + 1, (batch,), generator=g, device=DEV)
+    mask = torch.rand(batch, nk, generator=g, device=DEV) < 0.7
+    mask[1], mask[2, : nk // 2] = False, False
+    check(q, k, v, lengths=lengths)
+    check(q, k, v, lengths=lengths, window=50, sinks=3, key_mask=mask)
+    check(q, k, v, starts=lengths.int() - 20, window=50, causal=False, key_mask=mask, scale=-0.2)
+
+
+@pytest.mark.parametrize("nq", [17, 100, 256])
+@pytest.mark.parametrize("nk", [300, 5000])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (300, 40)])
+def test_some_queries_over_a_cache(nq, nk, window, sinks):
+    """Several row tiles of one K/V head, their keys split."""
+    for heads, kv in ((8, 1), (4, 2), (1, 1), (3, 1)):
+        q, k, v = heads_of(40, 1, nq, nk, heads, kv)
+        check(q, k, v, window=window, sinks=sinks)
+        check(q, k, v, window=window, sinks=sinks, causal=False, starts=max(nk - 2 * nq, 0))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_non_finite_values_in_hidden_places_of_many_items(causal, value):
+    batch, n = 20, 130
+    q, k, v = heads_of(41, batch, n, n, 8, 8)
+    mask = torch.ones(batch, n, device=DEV, dtype=torch.bool)
+    mask[0, 5:9], mask[1, 90:95], mask[5] = False, False, False
+    lengths = torch.full((batch,), n, device=DEV)
+    lengths[1], lengths[2], lengths[3] = n - 3, 0, 1
+    for window, sinks in ((None, 0), (60, 2)):
+        options = dict(window=window, sinks=sinks, causal=causal, key_mask=mask, lengths=lengths)
+        seen = visible(batch, n, n, window, sinks, causal, lengths, None, mask)
+        hidden = ~seen.any(1)[:, None, :, None]
+        check(q, k, v, K.window_attention(q, k.masked_fill(hidden, value), v.masked_fill(hidden, value), **options), **options)
+        vb = v.clone()
+        vb[:, :, 100, 3] = value
+        got = K.window_attention(q, k, vb, **options).unflatten(-1, (-1, 128))
+        touched = torch.zeros_like(got, dtype=torch.bool)
+        touched[..., 3] = seen[:, :, 100, None]
+        assert touched.any() and not torch.isfinite(got[touched]).any()
+        want, tol = reference(q, k, v, **options)
+        assert ((got.double() - want).abs() <= tol)[~touched].all()
+
+
+def test_many_rows_over_keys_that_span_two_gib():
+    rows, stride = 130, 9 << 20
+    flat = torch.empty(rows * stride, device=DEV, dtype=BF16)
+    k = flat.as_strided((1, 1, rows, 128), (rows * stride, 128, stride, 1))
+    v = flat.as_strided((1, 1, rows, 128), (rows * stride, 128, stride, 1), 256)
+    g = torch.Generator(device=DEV).manual_seed(42)
+    k.copy_(torch.randn(rows, 128, generator=g, device=DEV))
+    v.copy_(torch.randn(rows, 128, generator=g, device=DEV))
+    q = torch.randn(1, 70, 100, 128, generator=g, device=DEV).to(BF16)  # 438 row tiles
+    for options in (dict(window=30, sinks=2), dict(causal=False)):
+        check(q, k.contiguous(), v.contiguous(), K.window_attention(q, k, v, **options), **options)
