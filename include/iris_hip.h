@@ -209,7 +209,7 @@ typedef struct {
   long workspace_bytes;
 } iris_window_attn_args;
 int iris_window_attn(const iris_window_attn_args* args, hipStream_t stream);
-/* Bytes of workspace that iris_window_attn needs for these arguments (by shapes, window, sinks and causal alone). */
+/* Bytes of workspace that iris_window_attn needs for these arguments (by shapes, strides, window, sinks and causal). */
 int iris_window_attn_workspace(const iris_window_attn_args* args, long* bytes);
 
 /* mask.bool() of the encoder's [batch, >= n] attention mask (row stride ld elements) as the
