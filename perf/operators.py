@@ -24,18 +24,13 @@ own = False
 HD = 128  # attention's head width
 
 
-_loaded = None
-
-
 def _kernels():
-    """The framework's kernels, imported on the first call."""
-    global _loaded
-    if _loaded is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "iris-3b-metal_amd"))
-        from iris_mi355x import kernels
+    path = str(Path(__file__).resolve().parents[1] / "iris-3b-metal_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from iris_mi355x import kernels
 
-        _loaded = kernels
-    return _loaded
+    return kernels
 
 
 def listed() -> list[dict]:
