@@ -315,8 +315,8 @@ int iris_gemv_bf16_pair(const void* const* w, const float* x, int batch, const i
 int iris_timestep_gemv_bf16(const float* t, const float* freqs, int half, const void* w, int batch, int n,
                             const float* bias, float* out, int out_act, hipStream_t stream);
 
-/* One or two products (jobs) of the same inputs with 4-bit weights and group scales, in one launch (no
- * counterpart in the reference; beside iris_gemv_bf16 and its pair form):
+/* One or two products (jobs) of the same inputs with 4-bit weights and group scales, in one launch, or two
+ * where only one of them takes k in stages (no counterpart in the reference; beside iris_gemv_bf16 and its pair form):
  * W[n, k] = scales[n, k / group] (code[n, k] - zeros[n, k / group]), the code of an even k in the low half of
  * byte codes[n, k / 2] and of an odd k in the high half; zeros bytes 0..15, or null for 8 everywhere;
  * scales FP32 or BF16 [n, ceil(k / group)]. y[b, n] = act_out(sum_k W[n, k] act_in(x[b, k]) + bias[n]) with FP32

@@ -489,7 +489,7 @@ size_t plan_job(const W4Launch& a, W4Job& job, int& blocks, int depth) {
   return lds > sums ? lds : sums;
 }
 
-// Launches with DEPTH code loads underway, if that fits; 1 where it does not.
+// Launches with DEPTH code loads underway, if that fits; 1 where it does not. (staged: every product in stages of k.)
 template <typename X, int PARTS, int MT, int NT, int SPG, int DEPTH>
 int launch_depth(W4Launch& a, int jobs, bool staged, hipStream_t stream) {
   size_t lds = 0;
@@ -511,6 +511,21 @@ int launch_depth(W4Launch& a, int jobs, bool staged, hipStream_t stream) {
 
 template <typename X, int PARTS, int MT, int NT, int SPG>
 int launch_tiles(W4Launch& a, int jobs, hipStream_t stream) {
+  // A kernel in stages lays out what one round of its registers holds, one for all of k more than that: a product of
+  // each kind take a launch each.
+  if (jobs == 2) {
+    bool whole[2];
+    for (int j = 0; j < 2; ++j) {
+      int blocks;
+      whole[j] = plan_job<X, PARTS, MT, NT>(a, a.job[j], blocks, 1) && a.job[j].kc >= a.k;
+    }
+    if (whole[0] != whole[1]) {
+      W4Launch second = a;
+      second.job[0] = a.job[1];
+      const int rc = launch_tiles<X, PARTS, MT, NT, SPG>(a, 1, stream);
+      return rc ? rc : launch_tiles<X, PARTS, MT, NT, SPG>(second, 1, stream);
+    }
+  }
   // (more registers spill; with two workgroups on a CU two loads a wave do as well as four: 15360 x 5120 15.7 / 16.3 us)
   constexpr int kDepth = MT == 1 ? 4 : 2;
   int rc = launch_depth<X, PARTS, MT, NT, SPG, 2>(a, jobs, false, stream);

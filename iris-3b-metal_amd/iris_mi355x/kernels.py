@@ -1059,7 +1059,8 @@ def gemv_w4(
 def gemv_w4_pair(codes, scales, x: torch.Tensor, biases, outs, group: int = 64, zeros=(None, None),
                  extra_biases=(None, None), in_silu: bool = False, out_silu: bool = False) -> None:
     """Two ``gemv_w4`` of the same inputs in one launch (the image and text adaLN cores); same results as the
-    two calls. Scales, and outputs, share a dtype."""
+    two calls. Scales, and outputs, share a dtype. (Products of so different sizes that only one of them has all
+    of its inputs and scales in LDS at once take a launch each.)"""
     lists = (codes, scales, biases, outs, zeros, extra_biases)
     _Check("gemv_w4_pair")(all(len(items) == 2 for items in lists), "takes two products")
     jobs = [_w4_job("gemv_w4_pair", c, s, z, x, b, e, o, group) for c, s, b, o, z, e in zip(*lists)]

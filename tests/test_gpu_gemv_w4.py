@@ -228,3 +228,21 @@ def test_pair_of_which_one_takes_stages():
         K.gemv_w4(a[0], a[1], x, a[4], out, 64)
         assert torch.equal(got, out)
         check(got, (*a[:3], x, *a[4:]), 64)
+
+
+@pytest.mark.parametrize("batch,x_dtype,ns", [
+    (4, torch.float32, (30000, 40)), (5, torch.float32, (30000, 40)), (5, torch.float32, (40, 30000)),
+    (8, torch.bfloat16, (28672, 1024)), (9, torch.bfloat16, (28672, 1024)), (16, torch.bfloat16, (28672, 1024)),
+    (16, torch.bfloat16, (1024, 28672)), (16, torch.bfloat16, (15360, 1280))])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_pair_in_stages_is_two_calls(batch, x_dtype, ns, group):
+    """One product of a pair in stages of k, the other whole: with more inputs than a stage's first registers hold."""
+    jobs = [make(54 + i, n, 4096, group, batch, i == 1, x_dtype=x_dtype) for i, n in enumerate(ns)]
+    x = jobs[0][3]
+    outs = [[torch.full((batch, a[0].shape[0]), 7.0, device=DEV) for a in jobs] for _ in range(2)]
+    K.gemv_w4_pair([a[0] for a in jobs], [a[1] for a in jobs], x, [a[4] for a in jobs], outs[0], group,
+                   [a[2] for a in jobs])
+    for a, out, got in zip(jobs, outs[1], outs[0]):
+        K.gemv_w4(a[0], a[1], x, a[4], out, group, a[2])
+        assert torch.equal(got, out)
+        check(got, (*a[:3], x, *a[4:]), group)
