@@ -246,3 +246,53 @@ def test_pair_in_stages_is_two_calls(batch, x_dtype, ns, group):
         K.gemv_w4(a[0], a[1], x, a[4], out, group, a[2])
         assert torch.equal(got, out)
         check(got, (*a[:3], x, *a[4:]), group)
+
+
+def product_by_product(args, group, in_silu=False):
+    """The formula in FP64 with every infinity and NaN where it puts them."""
+    codes, scales, z, x, bias, _ = args
+    xd = torch.nn.functional.silu(x.double()) if in_silu else x.double()
+    return (xd[:, None, :] * weights(codes, scales, z, group)).sum(-1) + bias.double()
+
+
+@pytest.mark.parametrize("x_dtype,batch", [(torch.float32, 20), (torch.bfloat16, 40), (torch.bfloat16, 7)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("in_silu", [False, True])
+def test_non_finite_values_give_what_the_formula_has(x_dtype, batch, zeros, in_silu):
+    """Infinities of either sign by the signs of weights and inputs, NaN only where an infinity meets its opposite, a zero or
+    a NaN; in later pieces of the rows, in a short last group."""
+    args = make(55, 70, 288, 128, batch, zeros, x_dtype=x_dtype)
+    codes, scales, z, x, bias, _ = args
+    inf, nan = float("inf"), float("nan")
+    x[batch - 1, 100], x[batch - 2, 287] = inf, -inf
+    x[0, 3], x[0, 200] = inf, -inf
+    x[2, 7], x[batch - 4, 0] = nan, -inf
+    scales[7, 2], scales[9, 0], scales[11, 1] = inf, -inf, nan
+    want = product_by_product(args, 128, in_silu)
+    got = run(args, 128, torch.float32, in_silu=in_silu).double()
+    assert (want == inf).any() and (want == -inf).any() and want.isnan().any() and want.isfinite().any()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    _, tol = expected(*args, 128, in_silu=in_silu)
+    assert ((got - want).abs() <= tol)[want.isfinite()].all()
+
+
+@pytest.mark.parametrize("x_dtype,batch", [(torch.float32, 17), (torch.bfloat16, 33), (torch.bfloat16, 1)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("in_silu", [False, True])
+def test_finite_results_of_offset_products_that_overflow(x_dtype, batch, zeros, in_silu):
+    """Inputs around 1e37 of one sign with small scales: 32 of them times 16 leave FP32, the result does not.
+
+    Such results are FP32 sums, lane by lane, of k / 64 products and over 64 lanes, the weight and each product rounded once:
+    (k / 64 + 6 + 2) 2^-24 of their absolute sum, a few 2^-23 for silu."""
+    codes, scales, z, x, bias, _ = make(56, 70, 288, 128, batch, zeros, x_dtype=x_dtype)
+    x = ((1 + x.float().abs()) * 1e37).to(x_dtype)
+    scales = (0.01 * scales.float()).to(scales.dtype)
+    args = (codes, scales, z, x, bias, None)
+    assert 16 * x.double()[:, :32].sum(1).min() > torch.finfo(torch.float32).max
+    w = weights(codes, scales, z, 128)
+    want = x.double() @ w.T + bias.double()
+    tol = (13 + (16 if in_silu else 0)) * 2.0 ** -24 * (x.double() @ w.abs().T) + 2.0 ** -23 * want.abs()
+    assert want.abs().max() < torch.finfo(torch.float32).max
+    got = run(args, 128, torch.float32, in_silu=in_silu).double()
+    assert ((got - want).abs() <= tol).all()
