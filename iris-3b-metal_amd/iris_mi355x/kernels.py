@@ -1049,7 +1049,8 @@ def gemv_w4(
     ``codes``: uint8 ``[N, K / 2]``, the even k of a pair in the low half of its byte (``pack_w4``);
     ``scales``: FP32 or BF16 ``[N, ceil(K / group)]``; ``zeros``: uint8 of that shape with values 0..15, or
     None for 8 everywhere. K and ``group`` are multiples of 32; the last group may be short. Sums are FP32 and,
-    for FP32 inputs, of FP32 products. ``bias`` FP32 ``[N]``; ``out`` FP32 or BF16 ``[B, N]``; with
+    for FP32 inputs, of FP32 products; they hold ``x * code`` and ``x * zero`` apart (up to ``62 |x| scale`` a
+    weight), which their roundings are relative to. ``bias`` FP32 ``[N]``; ``out`` FP32 or BF16 ``[B, N]``; with
     ``extra_bias`` (``[J, N]``) ``out[j] = y + extra_bias[j]`` (``out``: ``[J, B, N]``)."""
     job = _w4_job("gemv_w4", codes, scales, zeros, x, bias, extra_bias, out, group)
     _w4_call("gemv_w4", job, x, out, scales, group, in_silu, out_silu, codes, scales, zeros, bias, extra_bias, out)

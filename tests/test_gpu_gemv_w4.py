@@ -296,3 +296,29 @@ def test_finite_results_of_offset_products_that_overflow(x_dtype, batch, zeros, 
     assert want.abs().max() < torch.finfo(torch.float32).max
     got = run(args, 128, torch.float32, in_silu=in_silu).double()
     assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("batch", [1, 2, 9, 33])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_codes_at_the_zero_point_under_large_inputs(batch, zeros):
+    """Most weights zero, inputs of one sign with a few far above the others: the sums of x (16 + code) and x (16 + zero),
+    which the bound of ``expected`` counts whatever their difference, cancel almost whole."""
+    codes, scales, z, x, bias, _ = make(57, 150, 1312, 32, batch, zeros)
+    g = torch.Generator(device=DEV).manual_seed(58)
+    of = torch.arange(1312, device=DEV) // 32
+    zero = z[:, of] if zeros else torch.full((150, 1312), 8, device=DEV, dtype=torch.uint8)
+    code = torch.stack([codes & 15, codes >> 4], -1).flatten(1)
+    code = torch.where(torch.rand(150, 1312, generator=g, device=DEV) < 0.9, zero, code)
+    codes = (code[:, 0::2] | code[:, 1::2] << 4).contiguous()
+    x = x.abs()
+    x[:, [3, 700, 1311]] *= torch.tensor([1e3, 1e4, 3e3], device=DEV)
+    args = (codes, scales, z, x, bias, None)
+    want, tol = expected(*args, 32)
+    got = run(args, 32).double()
+    assert ((got - want).abs() <= tol).all()
+    code[:, [3, 700, 1311]] = zero[:, [3, 700, 1311]]  # the large inputs meet zeros alone
+    codes = (code[:, 0::2] | code[:, 1::2] << 4).contiguous()
+    args = (codes, scales, z, x, bias, None)
+    want, tol = expected(*args, 32)
+    got = run(args, 32).double()
+    assert ((got - want).abs() <= tol).all()
