@@ -190,9 +190,9 @@ int iris_flash_attn_masked(const void* q, const void* k, const void* vt, int bat
  * |position - j| < window or j < sinks) and (key_mask null or key_mask[b * mask_stride + j] != 0); a row that
  * sees nothing is 0. lengths: null (n_k) or [batch], clamped to [0, n_k]; starts: [batch] of kind 1 or 3, the
  * value `start` (kind 4), or length_b - n_q (kind 0). Integer kinds: 1 int32, 3 int64. out BF16 [batch, n_q,
- * heads * 128], unit column stride, other strides multiples of 4. K and V of keys that no query sees are not
- * used. workspace: iris_window_attn_workspace(args) bytes, 16-byte aligned (null if that is 0); its contents
- * matter to no other call. */
+ * heads * 128], unit column stride, other strides multiples of 4 that keep its rows apart, apart from q, k and v.
+ * K and V of keys that no query sees are not used. workspace: iris_window_attn_workspace(args) bytes, 16-byte
+ * aligned (null if that is 0); its contents matter to no other call. */
 typedef struct {
   const void *q, *k, *v;
   void* out;

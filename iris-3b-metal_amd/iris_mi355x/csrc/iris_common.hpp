@@ -34,6 +34,74 @@ int check_launch(const char* what);
 
 inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
+// ---- memory that strided tensors touch -----------------------------------------
+// A tensor of runs of `run` contiguous bytes at p + sum_i j_i strides[i], 0 <= j_i < shape[i].
+struct StridedRuns {
+  const void* p;
+  int dims;
+  long shape[4], strides[4];  // strides in bytes, of either sign
+  long run;
+};
+inline StridedRuns strided_runs(const void* p, const long* shape, const long* strides, int dims, int size, long run) {
+  StridedRuns t{p, dims, {}, {}, run * size};
+  for (int i = 0; i < dims; ++i) t.shape[i] = shape[i], t.strides[i] = strides[i] * size;
+  return t;
+}
+
+// Whether two such tensors share a byte; with a == b, whether two runs of one tensor do. Exact: two runs share a byte
+// iff their addresses' difference, a sum of stride times index difference over the axes, lies within a run; searched
+// axis by axis from the largest stride down, where the smaller ones leave one or two index differences to try for
+// layouts in use. (A layout that leaves more than 2^14 in all counts as sharing.)
+inline bool share_memory(const StridedRuns& a, const StridedRuns& b) {
+  struct Term {
+    __int128 stride, lo, hi;
+  } t[8];
+  const bool self = &a == &b;
+  int n = 0;
+  auto axes = [&](const StridedRuns& x, bool minus) {
+    for (int i = 0; i < x.dims; ++i) {
+      if (x.shape[i] <= 0) return false;
+      if (x.shape[i] == 1 || (x.strides[i] == 0 && !self)) continue;
+      const __int128 last = x.shape[i] - 1, s = x.strides[i];
+      const bool down = (s < 0) != minus;
+      int k = n;  // (one term for both tensors' axes of a stride)
+      for (int j = 0; j < n && !self; ++j)
+        if (t[j].stride == (s < 0 ? -s : s)) k = j;
+      if (k == n) t[n++] = Term{s < 0 ? -s : s, 0, 0};
+      if (down || self) t[k].lo -= last;
+      if (!down || self) t[k].hi += last;
+    }
+    return true;
+  };
+  if (!axes(a, true) || (!self && !axes(b, false))) return false;  // (empty)
+  for (int i = 1; i < n; ++i)
+    for (int j = i; j > 0 && t[j].stride > t[j - 1].stride; --j) {
+      const Term x = t[j];
+      t[j] = t[j - 1], t[j - 1] = x;
+    }
+  __int128 least[9] = {}, most[9] = {};  // of the terms from i on
+  for (int i = n - 1; i >= 0; --i) least[i] = least[i + 1] + t[i].stride * t[i].lo, most[i] = most[i + 1] + t[i].stride * t[i].hi;
+  int budget = 1 << 14;
+  // whether the terms from i on can add up to a value in [lo, hi]; other: an index differs already
+  auto search = [&](auto&& again, int i, __int128 lo, __int128 hi, bool other) -> bool {
+    if (--budget < 0) return true;
+    if (i == n) return lo <= 0 && hi >= 0 && (other || !self);
+    if (most[i] < lo || least[i] > hi) return false;
+    __int128 from = t[i].lo, to = t[i].hi;
+    if (t[i].stride > 0) {
+      auto floor_div = [](__int128 x, __int128 y) { return x / y - (x % y < 0); };
+      const __int128 f = -floor_div(-(lo - most[i + 1]), t[i].stride), l = floor_div(hi - least[i + 1], t[i].stride);
+      from = f > from ? f : from, to = l < to ? l : to;
+    }
+    for (__int128 d = from; d <= to; ++d)
+      if (again(again, i + 1, lo - d * t[i].stride, hi - d * t[i].stride, other || d != 0)) return true;
+    return false;
+  };
+  // run of b at address difference x from a run of a: they meet for -b.run < x < a.run
+  const __int128 base = self ? 0 : static_cast<__int128>(reinterpret_cast<intptr_t>(b.p)) - reinterpret_cast<intptr_t>(a.p);
+  return search(search, 0, 1 - b.run - base, a.run - 1 - base, false);
+}
+
 // Compute units of the current device (launch shapes that place one workgroup per CU).
 inline int device_cus() {
   static int cached[64] = {};

@@ -746,6 +746,8 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   IRIS_REQUIRE((n_q == 1 || g.out_strides[1] >= heads * kHd) && (batch == 1 || g.out_strides[0] >= heads * kHd) &&
                    g.out_strides[0] % 4 == 0 && g.out_strides[1] % 4 == 0,
                "window_attn: output rows must not overlap, strides must be multiples of 4");
+  const StridedRuns out_rows = strided_runs(g.out, g.out_shape, g.out_strides, 2, 2, heads * kHd);
+  IRIS_REQUIRE(!share_memory(out_rows, out_rows), "window_attn: output rows must not overlap");
   uintptr_t o0, o1, x0, x1;
   extent(g.out, g.out_shape, g.out_strides, 3, &o0, &o1);
   const void* in[3] = {g.q, g.k, g.v};

@@ -288,3 +288,28 @@ def test_size_limits():
     head = (at, 1, tokens, 1, 64, 64 * tokens, 64, 64, 1, 1 << 50, 1, 1, tokens, 64, 64 * tokens, 64 * tokens, 64, 1)
     with pytest.raises(ValueError, match="too many"):
         _lib.call("iris_rotary", _lib.ROTARY_ARGS.pack(1, 1, 3, 0, *head, *(0,) * 36, at, 1, 0, 0, 0, 0, at, 32, 0, 0, 1.0), None)
+
+
+def window_workspace(out_shape, out_strides, heads=4):
+    """``iris_window_attn_workspace`` of a call with such an output: its checks of arguments, without a launch."""
+    batch, n_q, _ = out_shape
+    q = (batch, heads, n_q, 128, heads * n_q * 128, n_q * 128, 128, 1)
+    k = (batch, 1, 70, 128, 70 * 128, 70 * 128, 128, 1)
+    args = _lib.WINDOW_ATTN_ARGS.pack(1 << 20, 1 << 30, 1 << 31, 1 << 40, *q, *k, *k, *out_shape, *out_strides, 0, 0, 1, 0, 0,
+                                      0, 0, 0, 0, 0, 0.1, 0, 0)
+    need = ctypes.c_long()
+    _lib.call("iris_window_attn_workspace", args, ctypes.byref(need))
+
+
+@pytest.mark.parametrize("strides", [(512, 512), (1024, 512), (512, 1024), (1024, 1024), (1536, 1024), (516, 1020),
+                                     (5120, 516 * 5)])
+def test_window_attention_refuses_output_rows_that_overlap(strides):
+    """Items that lie fewer rows apart than they have, and rows of two items that meet in part."""
+    with pytest.raises(ValueError, match="overlap"):
+        window_workspace((3, 5, 512), (*strides, 1))
+
+
+@pytest.mark.parametrize("strides", [(2560, 512), (512, 1536), (516, 3 * 516), (1024, 4096), (1 << 40, 512), (4096, 680)])
+def test_window_attention_takes_output_rows_that_lie_apart(strides):
+    """Item or row major, with room between, and rows of items that interleave."""
+    window_workspace((3, 5, 512), (*strides, 1))
