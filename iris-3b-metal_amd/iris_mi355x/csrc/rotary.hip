@@ -222,6 +222,7 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
   IRIS_REQUIRE(g.positions_kind == 1 || g.positions_kind == 3, "rotary: positions are int32 (1) or int64 (3)");
   const int size = g.dtype == IRIS_F32 ? 4 : 2;
   RotaryArgs a{};
+  StridedRuns xs[kMaxTensors] = {}, outs[kMaxTensors] = {};
   for (int i = 0; i < g.tensors; ++i) {
     const iris_rotary_tensor& t = g.t[i];
     const long heads = t.x_shape[2], rows = t.out_shape[2];
@@ -248,8 +249,9 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
     a.heads_total += static_cast<int>(heads);
     if (batch == 0 || tokens == 0 || rows == 0) continue;
     IRIS_REQUIRE(t.x && t.out && g.positions && g.freqs && (!to_rows || g.rows), "rotary: null pointer");
-    IRIS_REQUIRE((batch == 1 || t.out_strides[0]) && (heads == 1 || t.out_strides[1]) && (rows == 1 || t.out_strides[2]),
-                 "rotary: output %d is an expanded tensor", i);
+    xs[i] = strided_runs(t.x, t.x_shape, t.x_strides, 3, size, dim);
+    outs[i] = strided_runs(t.out, t.out_shape, t.out_strides, 3, size, dim);
+    IRIS_REQUIRE(!share_memory(outs[i], outs[i]), "rotary: output %d is an expanded tensor, or its heads overlap", i);
     uintptr_t x0, x1, y0, y1;
     extent(t.x, t.x_shape, t.x_strides, 4, size, &x0, &x1);
     extent(t.out, t.out_shape, t.out_strides, 4, size, &y0, &y1);
@@ -260,11 +262,12 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
                  "rotary: output %d must be its input itself (as [B, H, N, D]) or lie apart from it", i);
   }
   if (batch == 0 || tokens == 0) return IRIS_OK;
-  // (tensors of one projection interleave, so their extents may meet; one tensor given twice is a mistake)
+  // (tensors of one projection interleave: their extents meet, their heads do not)
   for (int i = 0; i < g.tensors; ++i)
     for (int j = 0; j < g.tensors; ++j)
-      IRIS_REQUIRE(i == j || g.t[i].out_shape[2] == 0 || (g.t[i].out != g.t[j].x && g.t[i].out != g.t[j].out),
-                   "rotary: output %d is another tensor's input or output", i);
+      IRIS_REQUIRE(i == j || !outs[i].p || !outs[j].p ||
+                       (!share_memory(outs[i], xs[j]) && (j < i || !share_memory(outs[i], outs[j]))),
+                   "rotary: output %d shares memory with another tensor's input or output", i);
   a.tensors = static_cast<int>(g.tensors);
   a.tokens = tokens;
   a.head_dim = static_cast<int>(dim);

@@ -240,3 +240,24 @@ def test_in_place_with_axes_of_one(batch, n, heads):
     strides = [s if size > 1 else 4096 + i for i, (size, s) in enumerate(zip(x.transpose(1, 2).shape, x.transpose(1, 2).stride()))]
     K.rotary(x, None, positions, freqs, q_out=x.transpose(1, 2).as_strided((batch, heads, n, 64), strides))
     check(x.transpose(1, 2), before, positions, freqs, "half")
+
+
+@pytest.mark.parametrize("batch,n", [(1, 1), (2, 1), (3, 9)])
+def test_tensors_that_interleave(batch, n):
+    """Query and key heads rotated in place in one projection; K and V caches that alternate row by row and head by head."""
+    g = torch.Generator(device=DEV).manual_seed(18)
+    proj = torch.randn(batch, n + 2, 8, 64, generator=g, device=DEV).to(torch.bfloat16)[:, 1: n + 1]
+    q, k, v = proj[:, :, 0:4], proj[:, :, 4:6], proj[:, :, 6:8]
+    positions, (freqs, _) = torch.arange(n, device=DEV) + 5, tables.rotary_frequencies(64, 10000.0, DEV)
+    before = proj.clone()
+    K.rotary(q, k, positions, freqs, q_out=q.transpose(1, 2), k_out=k.transpose(1, 2))
+    check(q.transpose(1, 2), before[:, :, 0:4], positions, freqs, "half")
+    check(k.transpose(1, 2), before[:, :, 4:6], positions, freqs, "half")
+    assert torch.equal(v, before[:, :, 6:8])
+    for shape in ((batch, 20, 2, 2, 64), (batch, 20, 2, 2, 72)):
+        caches = torch.zeros(shape, device=DEV, dtype=torch.bfloat16)[..., :64]
+        for kc, vc in ((caches[:, :, 0], caches[:, :, 1]), (caches[:, :, :, 0], caches[:, :, :, 1])):
+            K.rotary_store(before[:, :, 0:4], before[:, :, 4:6], v, positions, freqs, kc.transpose(1, 2), vc.transpose(1, 2))
+            check(kc.transpose(1, 2)[:, :, 5: 5 + n], before[:, :, 4:6], positions, freqs, "half")
+            assert torch.equal(vc[:, 5: 5 + n], v) and not kc[:, :5].any() and not vc[:, 5 + n:].any()
+            caches.zero_()

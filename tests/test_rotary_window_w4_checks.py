@@ -313,3 +313,25 @@ def test_window_attention_refuses_output_rows_that_overlap(strides):
 def test_window_attention_takes_output_rows_that_lie_apart(strides):
     """Item or row major, with room between, and rows of items that interleave."""
     window_workspace((3, 5, 512), (*strides, 1))
+
+
+def test_rotary_refuses_outputs_that_share_memory_in_part(unplaced):
+    """An output that meets another tensor's input or output at another address than its first, and one whose own heads do."""
+    q, k, v = torch.zeros(2, 5, 2, 64), torch.zeros(2, 5, 2, 64), torch.zeros(2, 5, 2, 64)
+    args = (torch.zeros(5, dtype=torch.int64), torch.zeros(32, dtype=torch.float64))
+    store = torch.zeros(4096)
+    size = 2 * 2 * 5 * 64
+    one, two = store[:size].view(2, 2, 5, 64), store[size - 1: 2 * size - 1].view(2, 2, 5, 64)
+    for a, b in ((one, two), (two, one)):
+        with pytest.raises(ValueError, match="another tensor"):
+            K.rotary(q, k, *args, q_out=a, k_out=b)
+        with pytest.raises(ValueError, match="another tensor"):
+            K.rotary_store(q, k, v, *args, a, b)
+        with pytest.raises(ValueError, match="another tensor"):
+            K.rotary(q, a.transpose(1, 2), *args, q_out=b)
+    packed = torch.zeros(2, 5, 6, 64)  # the heads of a projection, off by one into another tensor's
+    with pytest.raises(ValueError, match="another tensor"):
+        K.rotary(packed[:, :, 0:2], k, *args, k_out=packed[:, :, 1:3].transpose(1, 2))
+    for strides in ((640, 320, 32, 1), (640, 32, 128, 1), (320, 320, 64, 1), (640, 256, 64, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            K.rotary(q, None, *args, q_out=store.as_strided((2, 2, 5, 64), strides))
