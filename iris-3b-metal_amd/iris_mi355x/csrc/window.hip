@@ -684,7 +684,7 @@ __global__ __launch_bounds__(256) void window_rows_kernel(WindowArgs p, long tot
     const float x = wave_sum(q0 * to_f32(kk[0]) + q1 * to_f32(kk[1])) * p.scale_log2;
     const float top = fmaxf(m, x);
     const float a = top == m ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-    const float e = __builtin_amdgcn_exp2f(x - top);
+    const float e = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - top);  // (also while top is -inf)
     m = top;
     l = l * a + e;
     o0 = o0 * a + e * to_f32(vv[0]);

@@ -342,3 +342,25 @@ def test_many_rows_over_keys_that_span_two_gib():
     q = torch.randn(1, 70, 100, 128, generator=g, device=DEV).to(BF16)  # 438 row tiles
     for options in (dict(window=30, sinks=2), dict(causal=False)):
         check(q, k.contiguous(), v.contiguous(), K.window_attention(q, k, v, **options), **options)
+
+
+@pytest.mark.parametrize("batch,heads,kv,nq,nk,apart", [(2, 4, 2, 1, 300, 128), (2, 4, 2, 40, 300, 128), (70, 8, 8, 130, 130, 128),
+                                                        (20, 8, 8, 130, 130, 128), (1, 4, 1, 1, 40, 1 << 26),
+                                                        (1, 4, 1, 40, 40, 1 << 26)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (30, 2)])
+def test_scores_of_minus_infinity(batch, heads, kv, nq, nk, apart, window, sinks):
+    """Keys whose scores are -inf weigh nothing, the first visible one of a row and the last among them: as if masked."""
+    q, k, v = heads_of(43, batch, nq, nk, heads, kv)
+    q[..., 3] = q[..., 3].abs() + 0.1
+    shown = torch.ones(batch, nk, device=DEV, dtype=torch.bool)
+    shown[:, [0, 1, nk // 2, nk - 3]] = False
+    low = k.clone()
+    low[..., 3].masked_fill_(~shown[:, None], -torch.inf)
+    if apart > 128:  # rows far apart
+        flat = torch.empty(nk * apart, device=DEV, dtype=BF16)
+        views = [flat.as_strided((1, 1, nk, 128), (nk * apart, 128, apart, 1), 256 * i) for i in range(2)]
+        views[0].copy_(low), views[1].copy_(v)
+        got = K.window_attention(q, *views, window, sinks)
+    else:
+        got = K.window_attention(q, low, v, window, sinks)
+    check(q, k, v, got, window=window, sinks=sinks, key_mask=shown)
