@@ -743,8 +743,8 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   p.vs_b = stride(g.v_shape, g.v_strides, 0), p.vs_h = stride(g.v_shape, g.v_strides, 1), p.vs_n = stride(g.v_shape, g.v_strides, 2);
   for (long x : {p.qs_b, p.qs_h, p.qs_n, p.ks_b, p.ks_h, p.ks_n, p.vs_b, p.vs_h, p.vs_n})
     IRIS_REQUIRE(x % 8 == 0 && x >= 0, "window_attn: strides must be multiples of 8 elements, and not negative");
-  IRIS_REQUIRE((n_q == 1 || g.out_strides[1] >= heads * kHd) && (batch == 1 || g.out_strides[0] >= heads * kHd) &&
-                   g.out_strides[0] % 4 == 0 && g.out_strides[1] % 4 == 0,
+  p.os_b = batch > 1 ? g.out_strides[0] : 0, p.os_n = n_q > 1 ? g.out_strides[1] : 0;
+  IRIS_REQUIRE((n_q == 1 || p.os_n >= heads * kHd) && (batch == 1 || p.os_b >= heads * kHd) && p.os_b % 4 == 0 && p.os_n % 4 == 0,
                "window_attn: output rows must not overlap, strides must be multiples of 4");
   const StridedRuns out_rows = strided_runs(g.out, g.out_shape, g.out_strides, 2, 2, heads * kHd);
   IRIS_REQUIRE(!share_memory(out_rows, out_rows), "window_attn: output rows must not overlap");
@@ -761,7 +761,6 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   p.k = static_cast<const bf16*>(g.k);
   p.v = static_cast<const bf16*>(g.v);
   p.out = static_cast<bf16*>(g.out);
-  p.os_b = g.out_strides[0], p.os_n = g.out_strides[1];
   p.batch = static_cast<int>(batch);
   p.heads = static_cast<int>(heads);
   p.kv_heads = static_cast<int>(kv_heads);

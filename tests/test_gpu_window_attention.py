@@ -364,3 +364,14 @@ def test_scores_of_minus_infinity(batch, heads, kv, nq, nk, apart, window, sinks
     else:
         got = K.window_attention(q, low, v, window, sinks)
     check(q, k, v, got, window=window, sinks=sinks, key_mask=shown)
+
+
+@pytest.mark.parametrize("batch,nq,strides", [(1, 5, (3, 260, 1)), (3, 1, (520, 7, 1)), (1, 1, (1, 1, 1)), (1, 600, (2, 256, 1))])
+def test_output_strides_of_axes_of_one_say_nothing(batch, nq, strides):
+    q, k, v = heads_of(44, batch, nq, 600, 2, 1)
+    store = torch.full((nq * 260 + batch * 520,), 7.0, device=DEV, dtype=BF16)
+    out = store.as_strided((batch, nq, 256), strides)
+    K.window_attention(q, k, v, 50, 2, out=out)
+    assert torch.equal(out, K.window_attention(q, k, v, 50, 2))
+    out.fill_(7.0)
+    assert (store == 7.0).all()

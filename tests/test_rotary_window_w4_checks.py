@@ -335,3 +335,9 @@ def test_rotary_refuses_outputs_that_share_memory_in_part(unplaced):
     for strides in ((640, 320, 32, 1), (640, 32, 128, 1), (320, 320, 64, 1), (640, 256, 64, 1)):
         with pytest.raises(ValueError, match="overlap"):
             K.rotary(q, None, *args, q_out=store.as_strided((2, 2, 5, 64), strides))
+
+
+@pytest.mark.parametrize("shape,strides", [((1, 5, 512), (3, 512, 1)), ((3, 1, 512), (516, 7, 1)), ((1, 1, 512), (-1, 2, 1)),
+                                           ((3, 1, 512), (1024, 512, 1))])
+def test_window_attention_takes_any_output_stride_of_an_axis_of_one(shape, strides):
+    window_workspace(shape, strides)
