@@ -81,6 +81,11 @@ inline bool share_memory(const StridedRuns& a, const StridedRuns& b) {
     }
   __int128 least[9] = {}, most[9] = {};  // of the terms from i on
   for (int i = n - 1; i >= 0; --i) least[i] = least[i + 1] + t[i].stride * t[i].lo, most[i] = most[i + 1] + t[i].stride * t[i].hi;
+  if (self) {  // (nested axes, without a search)
+    int i = 0;
+    while (i < n && t[i].stride >= most[i + 1] + a.run) ++i;
+    if (i == n) return false;
+  }
   int budget = 1 << 14;
   // whether the terms from i on can add up to a value in [lo, hi]; other: an index differs already
   auto search = [&](auto&& again, int i, __int128 lo, __int128 hi, bool other) -> bool {

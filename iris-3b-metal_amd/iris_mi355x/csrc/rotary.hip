@@ -38,7 +38,7 @@ struct RotaryTensor {
 };
 struct RotaryArgs {
   RotaryTensor t[kMaxTensors];
-  int tensors, heads_total;
+  int tensors;
   long tokens;
   int tok;  // tokens per workgroup
   int head_dim, pairs, interleaved;
@@ -198,16 +198,6 @@ void launch_rotary(const RotaryArgs& a, bool vector, int batch, hipStream_t stre
 
 using namespace iris;
 
-namespace {
-// First and one-past-last address of a tensor.
-void extent(const void* p, const long* shape, const long* strides, int dims, int size, uintptr_t* lo, uintptr_t* hi) {
-  long first = 0, last = 0;
-  for (int i = 0; i < dims; ++i) (strides[i] < 0 ? first : last) += (shape[i] - 1) * strides[i];
-  *lo = reinterpret_cast<uintptr_t>(p) + first * size;
-  *hi = reinterpret_cast<uintptr_t>(p) + (last + 1) * size;
-}
-}  // namespace
-
 extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
   IRIS_REQUIRE(args, "rotary: null pointer");
   const iris_rotary_args& g = *args;
@@ -246,19 +236,15 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
                           rows,
                           static_cast<int>(heads),
                           (i < g.turned ? kTurn : 0) | (to_rows ? kToRows : 0)};
-    a.heads_total += static_cast<int>(heads);
     if (batch == 0 || tokens == 0 || rows == 0) continue;
     IRIS_REQUIRE(t.x && t.out && g.positions && g.freqs && (!to_rows || g.rows), "rotary: null pointer");
     xs[i] = strided_runs(t.x, t.x_shape, t.x_strides, 3, size, dim);
     outs[i] = strided_runs(t.out, t.out_shape, t.out_strides, 3, size, dim);
     IRIS_REQUIRE(!share_memory(outs[i], outs[i]), "rotary: output %d is an expanded tensor, or its heads overlap", i);
-    uintptr_t x0, x1, y0, y1;
-    extent(t.x, t.x_shape, t.x_strides, 4, size, &x0, &x1);
-    extent(t.out, t.out_shape, t.out_strides, 4, size, &y0, &y1);
     const bool same = t.x == t.out && !to_rows && (batch == 1 || t.x_strides[0] == t.out_strides[0]) &&
                       (tokens == 1 || t.x_strides[1] == t.out_strides[2]) &&
                       (heads == 1 || t.x_strides[2] == t.out_strides[1]);
-    IRIS_REQUIRE(same || x1 <= y0 || y1 <= x0,
+    IRIS_REQUIRE(same || !share_memory(xs[i], outs[i]),
                  "rotary: output %d must be its input itself (as [B, H, N, D]) or lie apart from it", i);
   }
   if (batch == 0 || tokens == 0) return IRIS_OK;

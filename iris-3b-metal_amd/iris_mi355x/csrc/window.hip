@@ -703,13 +703,6 @@ __global__ __launch_bounds__(256) void window_rows_kernel(WindowArgs p, long tot
 using namespace iris;
 
 namespace {
-void extent(const void* p, const long* shape, const long* strides, int dims, uintptr_t* lo, uintptr_t* hi) {
-  long first = 0, last = 0;
-  for (int i = 0; i < dims; ++i) (strides[i] < 0 ? first : last) += (shape[i] - 1) * strides[i];
-  *lo = reinterpret_cast<uintptr_t>(p) + first * 2;
-  *hi = reinterpret_cast<uintptr_t>(p) + (last + 1) * 2;
-}
-
 // Checks the arguments and turns them into the kernels' form; p.batch stays 0 where there is nothing to do.
 int window_args(const iris_window_attn_args* args, WindowArgs& p) {
   IRIS_REQUIRE(args, "window_attn: null pointer");
@@ -748,15 +741,12 @@ int window_args(const iris_window_attn_args* args, WindowArgs& p) {
                "window_attn: output rows must not overlap, strides must be multiples of 4");
   const StridedRuns out_rows = strided_runs(g.out, g.out_shape, g.out_strides, 2, 2, heads * kHd);
   IRIS_REQUIRE(!share_memory(out_rows, out_rows), "window_attn: output rows must not overlap");
-  uintptr_t o0, o1, x0, x1;
-  extent(g.out, g.out_shape, g.out_strides, 3, &o0, &o1);
   const void* in[3] = {g.q, g.k, g.v};
   const long* shapes[3] = {g.q_shape, g.k_shape, g.v_shape};
   const long* strides[3] = {g.q_strides, g.k_strides, g.v_strides};
-  for (int i = 0; i < (n_k ? 3 : 1); ++i) {
-    extent(in[i], shapes[i], strides[i], 4, &x0, &x1);
-    IRIS_REQUIRE(o1 <= x0 || x1 <= o0, "window_attn: out must lie apart from q, k and v");
-  }
+  for (int i = 0; i < 3; ++i)
+    IRIS_REQUIRE(!share_memory(out_rows, strided_runs(in[i], shapes[i], strides[i], 3, 2, kHd)),
+                 "window_attn: out must lie apart from q, k and v");
   p.q = static_cast<const bf16*>(g.q);
   p.k = static_cast<const bf16*>(g.k);
   p.v = static_cast<const bf16*>(g.v);

@@ -261,3 +261,13 @@ def test_tensors_that_interleave(batch, n):
             check(kc.transpose(1, 2)[:, :, 5: 5 + n], before[:, :, 4:6], positions, freqs, "half")
             assert torch.equal(vc[:, 5: 5 + n], v) and not kc[:, :5].any() and not vc[:, 5 + n:].any()
             caches.zero_()
+
+
+def test_an_output_between_its_inputs_rows():
+    g = torch.Generator(device=DEV).manual_seed(19)
+    packed = torch.randn(2, 7, 4, 64, generator=g, device=DEV)
+    before = packed.clone()
+    positions, (freqs, _) = torch.arange(7, device=DEV) + 5, tables.rotary_frequencies(64, 10000.0, DEV)
+    K.rotary(packed[:, :, 0:2], None, positions, freqs, q_out=packed[:, :, 2:4].transpose(1, 2))
+    check(packed[:, :, 2:4].transpose(1, 2), before[:, :, 0:2], positions, freqs, "half")
+    assert torch.equal(packed[:, :, 0:2], before[:, :, 0:2])

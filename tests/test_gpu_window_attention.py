@@ -375,3 +375,17 @@ def test_output_strides_of_axes_of_one_say_nothing(batch, nq, strides):
     assert torch.equal(out, K.window_attention(q, k, v, 50, 2))
     out.fill_(7.0)
     assert (store == 7.0).all()
+
+
+@pytest.mark.parametrize("nq", [1, 70])
+def test_an_output_between_its_inputs_rows(nq):
+    """Query, key, value and output columns of one buffer: their rows alternate and do not meet."""
+    g = torch.Generator(device=DEV).manual_seed(45)
+    packed = torch.randn(2, nq, 8, 128, generator=g, device=DEV).to(BF16)
+    before = packed.clone().transpose(1, 2)
+    q, k, v = (packed.transpose(1, 2)[:, a:b] for a, b in ((0, 2), (2, 4), (6, 8)))
+    out = packed.view(2, nq, 1024)[:, :, 512:768]
+    K.window_attention(q, k, v, 30, 1, out=out)
+    check(before[:, 0:2], before[:, 2:4], before[:, 6:8], out, window=30, sinks=1)
+    after = packed.transpose(1, 2)
+    assert torch.equal(after[:, :4], before[:, :4]) and torch.equal(after[:, 6:], before[:, 6:])
