@@ -78,14 +78,7 @@ __device__ __forceinline__ void store_out4(TC* p, float v0, float v1, float v2, 
   store4(p, f32x4{v0, v1, v2, v3});
 }
 
-// s_waitcnt with only the vector-memory counter constrained (gfx9 encoding).
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
-}
-
-// Same, and also all LDS reads of this wave (lgkmcnt = 0).
+// wait_vmcnt, and also all LDS reads of this wave (lgkmcnt = 0).
 template <int N>
 __device__ __forceinline__ void wait_vmcnt_lgkm0() {
   static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");

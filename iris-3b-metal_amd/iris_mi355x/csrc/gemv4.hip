@@ -82,13 +82,6 @@ struct Divisor {
   }
 };
 
-// A barrier for what passes through LDS, which leaves loads from memory underway.
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // LDS of a launch: A rows of kc BF16 + 16 bytes (the 16 rows of a fragment read then start in distinct banks),
 // and per weight row and group of a stage the scale and the offset's BF16 pair, rows an odd number of pairs apart.
 __host__ __device__ __forceinline__ int x_stride(int kc) { return 2 * kc + 16; }

@@ -249,6 +249,20 @@ __device__ __forceinline__ int xcd_remap(int wg, int total) {
   return xcd * base + (xcd < rem ? xcd : rem) + local;
 }
 
+// s_waitcnt with only the vector-memory counter constrained (gfx9 encoding).
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+// A barrier for what passes through LDS, which leaves loads from memory underway.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Raw buffer resources: word 3 of a gfx9-family buffer descriptor (32-bit dwords, no swizzle).
 // A buffer load takes one 32-bit VGPR byte offset and an SGPR offset, and reads past the
 // resource's size return zeros instead of faulting.

@@ -81,19 +81,6 @@ __device__ __forceinline__ Span span_of(const WindowArgs& p, long pos, int lengt
   return s;
 }
 
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
-}
-
-// A barrier for what passes through LDS, which leaves loads from memory underway.
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // Lane i of 16 gets column i of the 4 x 16 block whose row j the lanes 4 j .. 4 j + 3 address, 8 bytes each.
 __device__ __forceinline__ bf16x4 read_tr(const char* p) {
   return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
@@ -369,13 +356,17 @@ __device__ __forceinline__ int mask_byte(const unsigned char* mask, int kv0, int
   return kv0 + lane < length ? mask[kv0 + lane] : 0;
 }
 
-template <int RB, int NW, int STAGES, int KVT, bool MASK>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void
+// Waves of a workgroup, keys of a tile and tiles of the ring.
+constexpr int kPromptWaves = 4, kPromptKeys = 64, kPromptStages = 2;
+
+template <int RB, bool MASK>
+__global__ __launch_bounds__(64 * kPromptWaves) __attribute__((amdgpu_waves_per_eu(2))) void
 window_attn_kernel(WindowArgs p) {
+  constexpr int NW = kPromptWaves, KVT = kPromptKeys, STAGES = kPromptStages;
   constexpr int STAGE = 2 * KVT * 256;  // bytes: K rows, then V rows
-  constexpr int LOADS = KVT / 16;       // 1 KB loads (4 rows) per fetching wave and operand; the first four waves fetch
+  constexpr int LOADS = KVT / 4 / NW;   // 1 KB loads (4 rows) per wave and operand
   constexpr int LPW = 2 * LOADS;
-  static_assert((KVT == 32 || KVT == 64) && STAGES >= 2 && (STAGES - 2) * LPW < 64, "pipeline");
+  static_assert(LOADS * 4 * NW == KVT && STAGES >= 2 && (STAGES - 2) * LPW < 64, "pipeline");
   // (the only LDS of the kernel: with a second object, a fence's included, the compiler waits for the prefetch before
   // every tile's reads)
   __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
@@ -423,7 +414,6 @@ window_attn_kernel(WindowArgs p) {
   }
   const __amdgpu_buffer_rsrc_t rk = rows_buffer(kh, length, p.ks_n), rv = rows_buffer(vh, length, p.vs_n);
   auto issue = [&](int t, int stage) {
-    if (NW != 4 && w >= 4) return;
     const int kv0 = tiles.key(t);
     const int ks = kv0 * static_cast<int>(p.ks_n) * 2, vs = kv0 * static_cast<int>(p.vs_n) * 2;
     bf16* kl = reinterpret_cast<bf16*>(lds + stage * STAGE);
@@ -831,13 +821,12 @@ extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t s
   if (plan == kRows) {
     window_rows_kernel<<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, stream>>>(p, rows);
   } else if (plan == kPrompt) {
-    constexpr int kWaves = 4;
     // 32 rows a wave (a K/V fragment read from LDS serves two MFMAs) where that leaves seven workgroups for four CUs,
     // else 16 (twice the workgroups). 20 query heads on 5 K/V heads, us, 32 / 16 rows: causal 300 tokens 13.1 / 9.4,
     // 1000: 26.8 / 21.8, two of 1000: 34.9 / 29.5, eight of 300 (400 workgroups of 32 rows): 19.3 / 19.1, 4352 (680):
     // 138 / 150; all of 4352 to all 211 / 226; 32 on 8 heads, four of 512 (512): 24.5 / 24.8
     auto groups = [&](int rb) {
-      p.rows_per_wg = 16 * rb * kWaves / p.hpw;
+      p.rows_per_wg = 16 * rb * kPromptWaves / p.hpw;
       p.n_qblocks = (p.n_q + p.rows_per_wg - 1) / p.rows_per_wg;
       return static_cast<long>(p.batch) * p.kv_heads * p.n_hgroups * p.n_qblocks;
     };
@@ -849,14 +838,14 @@ extern "C" int iris_window_attn(const iris_window_attn_args* args, hipStream_t s
     const dim3 grid(p.total_wg);
     if (few) {
       if (p.key_mask)
-        window_attn_kernel<1, kWaves, 2, 64, true><<<grid, 64 * kWaves, 0, stream>>>(p);
+        window_attn_kernel<1, true><<<grid, 64 * kPromptWaves, 0, stream>>>(p);
       else
-        window_attn_kernel<1, kWaves, 2, 64, false><<<grid, 64 * kWaves, 0, stream>>>(p);
+        window_attn_kernel<1, false><<<grid, 64 * kPromptWaves, 0, stream>>>(p);
     } else {
       if (p.key_mask)
-        window_attn_kernel<2, kWaves, 2, 64, true><<<grid, 64 * kWaves, 0, stream>>>(p);
+        window_attn_kernel<2, true><<<grid, 64 * kPromptWaves, 0, stream>>>(p);
       else
-        window_attn_kernel<2, kWaves, 2, 64, false><<<grid, 64 * kWaves, 0, stream>>>(p);
+        window_attn_kernel<2, false><<<grid, 64 * kPromptWaves, 0, stream>>>(p);
     }
   } else {
     const long need = window_workspace(p);
