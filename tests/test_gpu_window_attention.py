@@ -389,3 +389,102 @@ def test_an_output_between_its_inputs_rows(nq):
     check(before[:, 0:2], before[:, 2:4], before[:, 6:8], out, window=30, sinks=1)
     after = packed.transpose(1, 2)
     assert torch.equal(after[:, :4], before[:, :4]) and torch.equal(after[:, 6:], before[:, 6:])
+
+
+def check_norm(q, k, v, got, **options):
+    """``check``, and a bound on the norm of the whole error, which leaves no room for a tile of keys left out or seen twice.
+
+    The output's rounding is at most 2^-8 of each element. The weights' are at most 2^-8 of each and independent of one
+    another: their sum over the keys has a mean square of at most (2^-16 / 3) sum w^2 v^2, and over a call's rows and dims
+    its norm stays below sqrt(3) times the root of that. The FP32 terms are those of ``reference``, at their worst."""
+    check(q, k, v, got, **options)
+    group = q.shape[1] // k.shape[1]
+    scale = options.pop("scale", None)
+    seen = visible(q.shape[0], q.shape[2], k.shape[2], *(options.get(name, default) for name, default in (
+        ("window", None), ("sinks", 0), ("causal", True), ("lengths", None), ("starts", None), ("key_mask", None))))[:, None]
+    some = seen.any(2)[:, :, :, None]
+    kd, vd = (torch.where(some, t.double().repeat_interleave(group, 1), 0.0) for t in (k, v))
+    s = q.double() @ kd.transpose(-1, -2) * (128 ** -0.5 if scale is None else scale)
+    w = torch.where(seen.any(-1, True), torch.softmax(s.masked_fill(~seen, -torch.inf), -1), 0.0)
+    o = w @ vd
+    off = q.double().norm(dim=-1).max() * kd.norm(dim=-1).max() * 128 ** -0.5 * 128 * 2.0 ** -24
+    bound = 2.0 ** -8 * (o.norm() + (w.square() @ vd.square()).sum().sqrt())
+    bound = bound + (2 * off + (k.shape[2] + 16) * 2.0 ** -24) * (w @ vd.abs()).norm()
+    err = got.unflatten(-1, (-1, 128)).double() - o.transpose(1, 2)
+    assert err.norm() <= bound, f"{(err.norm() / bound).item():.3g} of the norm's bound"
+
+
+# Calls of more workgroups of 32 rows a wave than seven for four CUs: a wave holds two blocks of 16 rows.
+@pytest.mark.parametrize("heads,kv", [(8, 8), (16, 8), (32, 8), (5, 5), (20, 5)])
+@pytest.mark.parametrize("n", [17, 31, 32, 33, 48, 64, 65, 96, 130, 200])
+@pytest.mark.parametrize("causal", [True, False])
+def test_two_row_blocks(heads, kv, n, causal):
+    batch = 64 if kv == 8 else 100  # (at least 500 workgroups at 32 rows of a head)
+    q, k, v = heads_of(46, batch, n, n, heads, kv, gain=2.0)
+    g = torch.Generator(device=DEV).manual_seed(47)
+    lengths = torch.randint(0, n + 1, (batch,), generator=g, device=DEV)
+    mask = torch.rand(batch, n, generator=g, device=DEV) < 0.7
+    mask[1], mask[2, : n // 2] = False, False
+    for options in (dict(), dict(window=20, sinks=3), dict(window=1), dict(window=40, sinks=70, key_mask=mask),
+                    dict(lengths=lengths, starts=0), dict(lengths=lengths, starts=lengths - 9, window=17, key_mask=mask)):
+        check_norm(q, k, v, K.window_attention(q, k, v, causal=causal, **options), causal=causal, **options)
+
+
+@pytest.mark.parametrize("nq,nk", [(17, 300), (40, 129), (64, 500), (130, 257)])
+@pytest.mark.parametrize("heads,kv", [(8, 8), (32, 8)])
+def test_two_row_blocks_over_a_cache(nq, nk, heads, kv):
+    """Query blocks whose windows end in different tiles; a negative scale; a strided output."""
+    q, k, v = heads_of(48, 64, nq, nk, heads, kv)
+    store = torch.full((64, nq, heads * 128 + 8), 7.0, device=DEV, dtype=BF16)
+    out = store[:, :, 4:-4]
+    for options in (dict(), dict(window=50, sinks=5), dict(window=65, causal=False, starts=nk // 3),
+                    dict(window=nk // 2, scale=-0.15, starts=-5, causal=False)):
+        check_norm(q, k, v, K.window_attention(q, k, v, out=out, **options), **options)
+    out.fill_(7.0)
+    assert (store == 7.0).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("at", [3, 20, 70, 100])
+def test_non_finite_values_in_hidden_places_of_two_row_blocks(causal, value, at):
+    batch, n = 64, 130
+    q, k, v = heads_of(49, batch, n, n, 8, 8)
+    mask = torch.ones(batch, n, device=DEV, dtype=torch.bool)
+    mask[0, 5:9], mask[1, 90:95], mask[5] = False, False, False
+    lengths = torch.full((batch,), n, device=DEV)
+    lengths[1], lengths[2], lengths[3] = n - 3, 0, 1
+    for window, sinks in ((None, 0), (60, 2)):
+        options = dict(window=window, sinks=sinks, causal=causal, key_mask=mask, lengths=lengths)
+        seen = visible(batch, n, n, window, sinks, causal, lengths, None, mask)
+        hidden = ~seen.any(1)[:, None, :, None]
+        got = K.window_attention(q, k.masked_fill(hidden, value), v.masked_fill(hidden, value), **options)
+        check_norm(q, k, v, got, **options)
+        vb = v.clone()
+        vb[:, :, at, 3] = value
+        got = K.window_attention(q, k, vb, **options).unflatten(-1, (-1, 128))
+        touched = torch.zeros_like(got, dtype=torch.bool)
+        touched[..., 3] = seen[:, :, at, None]
+        assert touched.any() and not torch.isfinite(got[touched]).any()
+        want, tol = reference(q, k, v, **options)
+        assert ((got.double() - want).abs() <= tol)[~touched].all()
+        kb = k.clone()
+        kb[:, :, at, 7] = value
+        got = K.window_attention(q, kb, v, **options).unflatten(-1, (-1, 128))
+        assert ((got.double() - want).abs() <= tol)[~seen[:, :, at]].all()
+
+
+@pytest.mark.parametrize("batch,nq,nk", [(1, 1, 16385), (2, 1, 40000), (7, 1, 20000), (1, 2, 40000), (1, 16, 32768), (1, 128, 16384)])
+@pytest.mark.parametrize("heads,kv", [(8, 2), (20, 5)])
+def test_long_caches_in_norm(batch, nq, nk, heads, kv):
+    """A 32-key tile left out of 40000 keys would be 3 % of the output, three times the bound."""
+    q, k, v = heads_of(50, batch, nq, nk, heads, kv)
+    for options in (dict(), dict(window=nk // 2, sinks=100)):
+        check_norm(q, k, v, K.window_attention(q, k, v, **options), **options)
+
+
+@pytest.mark.parametrize("nq,nk", [(1, 300), (3, 1000), (40, 200), (300, 300), (1000, 1000)])
+def test_prompts_and_caches_in_norm(nq, nk):
+    q, k, v = heads_of(51, 4, nq, nk, 20, 5, gain=1.5)
+    for options in (dict(), dict(window=100, sinks=4), dict(window=33, causal=False)):
+        check_norm(q, k, v, K.window_attention(q, k, v, **options), **options)
