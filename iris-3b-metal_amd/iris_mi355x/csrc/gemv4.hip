@@ -15,8 +15,7 @@
 //   What the FP32 sums hold is thus x (16 + code) and -x (16 + zero), up to 62 |x| scale a weight whatever
 //   code - zero is, and their roundings are to that: an input far above the others leaves about 2^-24 of it
 //   times 24 scale in results that its weight, a zero, has no part in (inputs of 1000 to 10000 among ones of 1,
-//   meeting zeros alone in 1312 x 150 weights: 2e-4 of the result in norm; where they do take part, and for
-//   codes and inputs without such places, 1e-7).
+//   meeting zeros alone in 1312 x 150 weights: up to 2e-4 of the result in norm; without such inputs 0.9e-7).
 // - A: BF16 rows as they are; FP32 rows (and activated ones) as three BF16 rows that add up to them exactly
 //   (8 + 8 + 8 bits of significand, by truncation; below 2^-110 the last row's steps of 2^-133 cut them off), so
 //   FP32 inputs keep FP32 products at no extra MFMA while
@@ -26,8 +25,10 @@
 // A workgroup's eight waves are dealt over weight tiles and over k (their sums joined in LDS): many tiles where
 // the weight has rows enough for all CUs, because every workgroup lays out all inputs anew, few where it has not.
 // One row, 131072 x 4096: 60 us, 4.6 TB/s (a large copy moves 4.9). Small calls are bound by their chain of latencies:
-// inputs and scales to LDS, products, the join of the waves, the store: 6.3 us for 2560 x 2560 of which a launch that
-// does nothing takes about 3; 11.9 us for two FP32 rows, 15360 x 2560, 24 outputs; 14.8 us for 24 rows, 13696 x 2560.
+// inputs and scales to LDS, products, the join of the waves, the store: 6.2 us for 2560 x 2560 of which a launch that
+// does nothing takes about 3; 12.0 us for two FP32 rows, 15360 x 2560, 24 outputs (VALU issue 26 % of the waves' cycles,
+// the matrix cores busy 10 %); 15.1 us for 24 rows, 13696 x 2560 (26 and 15 %). More rows than a workgroup holds read and
+// unpack all codes once per piece: 13696 x 2560, BF16 32 rows 17 us, 33: 23, 64: 32; FP32 16 rows 20, 17: 24, 64: 73.
 #include "iris_common.hpp"
 
 namespace iris {

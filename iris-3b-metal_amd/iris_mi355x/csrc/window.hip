@@ -15,12 +15,16 @@
 //
 // window_attn_kernel (prompts): bound by the MFMAs and the softmax beside them. A workgroup's waves share a
 // ring of K/V tiles; a wave is one query head's 16 or 32 rows, the heads of a K/V head side by side. 8192 tokens, 32 on 8
-// heads, window 4096: 391 us, 1054 TFLOP/s of visible pairs; 4352 tokens, 20 on 5, two-sided window 640 and 256 first
-// keys: 88 us, 705 TFLOP/s (680 workgroups in 512 places); small prompts are a chain of 5 us and 0.8 us per tile.
+// heads, window 4096: 398 us, 1037 TFLOP/s of visible pairs, the matrix cores busy 51 % of the cycles in which a CU holds
+// waves and a wave issuing VALU 27 % of its own; 4352 tokens, 20 on 5, two-sided window 640 and 256 first keys: 87 us, 713
+// TFLOP/s (680 workgroups in 512 places: CUs hold waves for 68 % of the launch); small prompts are a chain of 5 us and
+// 0.8 us per tile. (Replayed in a graph; a profiler's single launches take 434 and 97 us.)
 // window_few_kernel (few queries): bound by the keys' and values' way from memory. The rows of a tile are the
 // (query, head) pairs of one K/V head; every wave streams key tiles of its own through its own LDS, without
 // barriers, and the waves' and workgroups' parts are joined at the end (window_join_kernel for the latter). 16 queries
-// of 32 on 8 heads over 65536 keys at most: 599 us, 5.5 TB/s; one query over 1028 keys: 11 us in two launches.
+// of 32 on 8 heads over 65536 keys at most: 598 us, 5.5 TB/s; one query over 1028 keys: 11 us in two launches. Several row
+// tiles of a K/V head each read its keys: 16 queries of 20 on 5 heads over a cache of 32768 keys 45 us, 32: 98, where K
+// and V read once are 17.
 // window_rows_kernel: row strides of 2^24 elements and more, too large for the 32-bit offsets of the others.
 #include "iris_common.hpp"
 
@@ -235,7 +239,8 @@ struct Attend {
     // up to at most 2^8 the maximum and the output stay as they are; otherwise the queries that need it take their
     // exact maxima, rescale, and recompute. A query with no key so far keeps -inf, and its hidden keys are taken
     // against 0, which makes them exact zeros instead of NaN. The sums add the FP32 exponentials; P is rounded to
-    // BF16 (the MFMA's operand) after that.
+    // BF16 (the MFMA's operand; a second one for the rest would double the P V products) after that: up to 2^-8 of
+    // each weight, and 0.0020 to 0.0023 from a 64-bit result in norm where FP32 weights leave 0.0016, the output's rounding.
     bf16x8 pf[H32][RB];
     auto probs = [&](int qb, float ref) {
       float sum = 0.0f;
@@ -769,9 +774,9 @@ int window_plan(WindowArgs& p) {
   p.row_tiles = (rows + 15) / 16;
   const long base = static_cast<long>(p.batch) * p.kv_heads * p.row_tiles, cus = device_cus();
   // Few: no more 16-row tiles than CUs, so that the prompts' form, a wave for 16 rows of a head with all of its keys,
-  // would leave most waves of the card without work. us, few / prompts: 20 on 5 heads, 16 queries of 32768 keys 68 / 605, 32:
-  // 101 / 575, 64 of 4096 keys: 26 / 61, 128 of 1000 (160 tiles): 16 / 18, of 16384: 135 / 224; 8 on 1 head, 400 of 1000
-  // (200): 15.5 / 18; beyond: 32 items of 16 queries, 1024 keys (640) 49 / 27; 64 items of one query, 2048 keys (320)
+  // would leave most waves of the card without work. us, few / prompts (heads of packed rows): 20 on 5 heads, 16 queries of
+  // 32768 keys 68 / 605, 32: 101 / 575, 64 of 4096 keys: 26 / 61, 128 of 1000 (160 tiles): 16 / 18, of 16384: 135 / 224;
+  // 8 on 1 head, 400 of 1000 (200): 15.5 / 18; beyond: 32 items of 16 queries, 1024 keys (640) 49 / 27; 64 items of one query, 2048 keys (320)
   // 81 / 68. (The prompts' form reaches all rows by 32-bit offsets; this one those of a tile.)
   if (base > cus && (p.n_k + 64) * (p.ks_n > p.vs_n ? p.ks_n : p.vs_n) * 2 < (1L << 31)) return kPrompt;
   // keys that a tile's queries can see at most, in tiles

@@ -96,7 +96,8 @@ class HipIris:
 
     ``core_bits=4`` keeps the two shared adaLN cores, every step's largest read beside the blocks, in 4
     bits (``kernels.pack_w4``, groups of 64) instead of BF16: a quarter of their memory and traffic, and
-    modulation vectors of the rounded weights.
+    modulation vectors of the rounded weights. (Their launch takes 15.5 us instead of 33; a 1024 x 1024
+    forward 21.85 ms with either.)
     """
 
     def __init__(self, cfg: ModelConfig, state_dict: dict[str, torch.Tensor], device: str | torch.device = "cuda",
