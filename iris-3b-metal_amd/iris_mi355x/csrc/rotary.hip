@@ -238,8 +238,9 @@ extern "C" int iris_rotary(const iris_rotary_args* args, hipStream_t stream) {
                           rows,
                           static_cast<int>(heads),
                           (i < g.turned ? kTurn : 0) | (to_rows ? kToRows : 0)};
-    if (batch == 0 || tokens == 0 || rows == 0) continue;
-    IRIS_REQUIRE(t.x && t.out && g.positions && g.freqs && (!to_rows || g.rows), "rotary: null pointer");
+    if (batch == 0 || tokens == 0) continue;
+    IRIS_REQUIRE(t.x && (t.out || rows == 0) && g.positions && g.freqs && (!to_rows || g.rows), "rotary: null pointer");
+    if (rows == 0) continue;  // (read all the same, and dropped)
     xs[i] = strided_runs(t.x, t.x_shape, t.x_strides, 3, size, dim);
     outs[i] = strided_runs(t.out, t.out_shape, t.out_strides, 3, size, dim);
     IRIS_REQUIRE(!share_memory(outs[i], outs[i]), "rotary: output %d is an expanded tensor, or its heads overlap", i);

@@ -271,3 +271,11 @@ def test_an_output_between_its_inputs_rows():
     K.rotary(packed[:, :, 0:2], None, positions, freqs, q_out=packed[:, :, 2:4].transpose(1, 2))
     check(packed[:, :, 2:4].transpose(1, 2), before[:, :, 0:2], positions, freqs, "half")
     assert torch.equal(packed[:, :, 0:2], before[:, :, 0:2])
+
+
+def test_caches_without_rows():
+    g = torch.Generator(device=DEV).manual_seed(20)
+    q, k, v = (torch.randn(2, 5, h, 64, generator=g, device=DEV) for h in (4, 2, 2))
+    positions, (freqs, _) = torch.arange(5, device=DEV), tables.rotary_frequencies(64, 10000.0, DEV)
+    caches = [torch.empty(2, 2, 0, 64, device=DEV) for _ in range(2)]
+    check(K.rotary_store(q, k, v, positions, freqs, *caches), q, positions, freqs, "half")

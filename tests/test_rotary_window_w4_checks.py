@@ -341,3 +341,13 @@ def test_rotary_refuses_outputs_that_share_memory_in_part(unplaced):
                                            ((3, 1, 512), (1024, 512, 1))])
 def test_window_attention_takes_any_output_stride_of_an_axis_of_one(shape, strides):
     window_workspace(shape, strides)
+
+
+@pytest.mark.parametrize("x,positions,freqs,rows_at", [(0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0)])
+def test_rotary_refuses_null_inputs_of_an_output_without_rows(x, positions, freqs, rows_at):
+    """Heads for a cache of no rows are read before their rows are found not to exist."""
+    at = 1 << 20
+    head = (x * at, 2, 5, 2, 64, 640, 128, 64, 1, 0, 2, 2, 0, 64, 0, 0, 64, 1)
+    args = _lib.ROTARY_ARGS.pack(1, 1, 0, 0, *head, *(0,) * 36, positions * at, 1, 5, rows_at * at, 1, 5, freqs * at, 32, 0, 0, 1.0)
+    with pytest.raises(ValueError, match="null"):
+        _lib.call("iris_rotary", args, None)
